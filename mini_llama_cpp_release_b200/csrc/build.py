@@ -33,9 +33,11 @@ NVCC_FLAGS = [
 ]
 
 # library name → (sources, extra -D flags may be added per variant)
-CORE_SOURCES = ["elementwise.cu", "attention_simt.cu", "sampling.cu", "linear_simt.cu", "recurrent.cu", "linear_attention.cu", "gla_chunks.cu", "matrix_memory.cu", "rms_pair.cu", "latent.cu", "mixture.cu", "group_norm.cu", "tanh_norm.cu", "gemm_few.cu", "gemm_few_grouped.cu", "gemm_tcgen05.cu", "gemm_tcgen05_rows.cu", "gemm_tcgen05_pair.cu"]
+CORE_SOURCES = ["elementwise.cu", "attention_simt.cu", "sampling.cu", "linear_simt.cu", "recurrent.cu", "linear_attention.cu", "gla_chunks.cu", "matrix_memory.cu", "rms_pair.cu", "latent.cu", "mixture.cu", "group_norm.cu", "tanh_norm.cu", "gemm_few.cu", "gemm_few_grouped.cu", "gemm_tcgen05.cu", "gemm_tcgen05_rows.cu", "gemm_tcgen05_pair.cu", "kv_quantise.cu"]
 # compiled once per head size (-DMLC_HEAD_DIM=...): the mma.sync kernels for every size, the tcgen05 kernel for 64 and 128
 ATTENTION_SOURCES = ["attention_mma.cu", "attention_tcgen05.cu"]
+# the same over an 8-bit cache, built when a cache of that kind is asked for
+ATTENTION_Q8_SOURCES = ["attention_q8.cu"]
 
 _lock = threading.Lock()
 _loaded: Dict[str, ctypes.CDLL] = {}
@@ -183,6 +185,13 @@ def attention_library(head_dim: int) -> ctypes.CDLL:
     return load_library(f"mlc_attn_hd{head_dim}", ATTENTION_SOURCES, [f"-DMLC_HEAD_DIM={head_dim}"])
 
 
+def attention_q8_library(head_dim: int) -> ctypes.CDLL:
+    """The attention kernels over an 8-bit cache, compiled for one head size."""
+    if head_dim % 16 != 0 or not 16 <= head_dim <= 256:
+        raise BuildError(f"the attention kernels over an 8-bit cache take head sizes 16, 32, ..., 256; got {head_dim}")
+    return load_library(f"mlc_attn_q8_hd{head_dim}", ATTENTION_Q8_SOURCES, [f"-DMLC_HEAD_DIM={head_dim}"])
+
+
 def noalloc_library() -> ctypes.CDLL:
     """The allocation-free attention entry point (csrc/attention_noalloc.h), a library of its
     own so that only processes that ask for it hold its fixed scratch array."""
@@ -195,4 +204,5 @@ def build_everything(head_dims: Iterable[int] = (16, 64, 128)) -> List[str]:
     if os.path.exists(os.path.join(_HERE, "attention_mma.cu")):
         for hd in head_dims:
             paths.append(build_library(f"mlc_attn_hd{hd}", ATTENTION_SOURCES, [f"-DMLC_HEAD_DIM={hd}"]))
+            paths.append(build_library(f"mlc_attn_q8_hd{hd}", ATTENTION_Q8_SOURCES, [f"-DMLC_HEAD_DIM={hd}"]))
     return paths

@@ -22,6 +22,7 @@ __all__ = [
     "group_norm", "activation", "forget_gate_attention", "moe_route_scored",
     "tanh_norm", "glu", "sigmoid_gate", "state_space",
     "decay_attention", "matrix_memory", "rms_pair", "embed_rms", "diff_combine", "moe_plan_table",
+    "QuantisedKVView", "quantise_kv", "dequantise_kv", "attention_quantised", "attention_q8_library", "attention_q8_plan",
 ]
 
 
@@ -146,6 +147,8 @@ def core() -> ctypes.CDLL:
             "mlc_argmax_split": [P, I, I, P, P, P, P, P],
             "mlc_sample": [P, I, I, F, I, c_ulonglong, P, P, P, P, P],
             "mlc_decode_advance": [P, I, P, P, P, P, P, P, I, P],
+            "mlc_quantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, P, P, P, P, P, I, I, LL, LL, I, I, I, P],
+            "mlc_dequantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, P, P, P, P, P, I, I, LL, LL, I, I, I, P],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)
@@ -1347,7 +1350,8 @@ def check_gemm_status(device: torch.device) -> None:
                    21: "the prompt product's TMA loader", 22: "the prompt product's tensor-core issuer",
                    23: "the prompt product's epilogue", 31: "the single-token attention kernel's wait for keys and values", 41: "the paired prompt product's TMA loader",
                    42: "the paired prompt product's tensor-core issuer or relay", 43: "the paired prompt product's epilogue",
-                   61: "the float32 few-row product's wait for its operands"}.get(code, str(code))
+                   61: "the float32 few-row product's wait for its operands", 71: "the 8-bit cache attention's loader",
+                   72: "the 8-bit cache attention's wait for keys and values"}.get(code, str(code))
             raise KernelError(f"a tcgen05 kernel gave up waiting on a barrier ({who}); its output is not valid")
 
 
@@ -1771,3 +1775,175 @@ def gemm_tcgen05(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, epilogue: 
                                    _ptr(bias), _ptr(positions),
                                    _ptr(tok_seq), _ptr(rope), rope.shape[0] if rope is not None else 0, q_heads,
                                    kv_heads, head_dim, *cache, *_glu_args(glu), _stream()), "tcgen05 matrix product")
+
+
+# ------------------------------------------------------------------ the 8-bit cache
+
+@dataclass
+class QuantisedKVView:
+    """Where one cache entry's keys and values are in an 8-bit cache: pools of e4m3 numbers
+    [entries][pages][kv_heads][page_size][head_dim] and of their rows' scale bytes [entries][pages][kv_heads][page_size] (byte b
+    stands for 2^(b - 127)), the entry's offset in numbers, and the page lists [n_seqs][pages_per_seq] of the sequences of
+    this step (-1: no page).  An entry whose values are read out of its key rows has the same pools under both names."""
+    k_pool: torch.Tensor
+    v_pool: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    entry_offset: int
+    page_table: torch.Tensor
+    page_size: int
+    kv_heads: int
+    head_dim: int
+
+    @property
+    def pages_per_seq(self) -> int:
+        return self.page_table.shape[1]
+
+
+def _check_quantised(kv: QuantisedKVView, *others: Optional[torch.Tensor]) -> None:
+    """What a kernel cannot see for itself: types, devices, and that pools, scales and offset belong together."""
+    device = kv.k_pool.device
+    if device.type != "cuda":
+        raise KernelError("this engine runs on a CUDA device only: got a cache on " + str(device))
+    if device.index != torch.cuda.current_device():
+        raise KernelError(f"the cache lies on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in (kv.v_pool, kv.k_scale, kv.v_scale, kv.page_table) + others:
+        if t is not None and t.device != device:
+            raise KernelError(f"tensors on different devices: {t.device} and {device}")
+    if kv.k_pool.dtype != torch.float8_e4m3fn or kv.v_pool.dtype != torch.float8_e4m3fn:
+        raise KernelError(f"an 8-bit cache holds float8_e4m3fn, not {kv.k_pool.dtype} and {kv.v_pool.dtype}")
+    if kv.k_scale.dtype != torch.uint8 or kv.v_scale.dtype != torch.uint8:
+        raise KernelError("the scales of an 8-bit cache are bytes (uint8)")
+    shape = kv.k_pool.shape
+    if len(shape) != 5 or tuple(shape[2:]) != (kv.kv_heads, kv.page_size, kv.head_dim) or kv.v_pool.shape != shape \
+            or kv.k_scale.shape != shape[:4] or kv.v_scale.shape != shape[:4]:
+        raise KernelError(f"pools {tuple(shape)}, {tuple(kv.v_pool.shape)} and scales {tuple(kv.k_scale.shape)}, {tuple(kv.v_scale.shape)} do not "
+                          f"fit {kv.kv_heads} kv heads, pages of {kv.page_size} and heads of {kv.head_dim}")
+    per_entry = shape[1] * kv.kv_heads * kv.page_size * kv.head_dim
+    if not (kv.k_pool.is_contiguous() and kv.v_pool.is_contiguous() and kv.k_scale.is_contiguous() and kv.v_scale.is_contiguous()):
+        raise KernelError("the pools of an 8-bit cache are dense")
+    if kv.entry_offset < 0 or (per_entry and (kv.entry_offset % per_entry or kv.entry_offset // per_entry >= shape[0])):
+        raise KernelError(f"an entry starts at a multiple of {per_entry} numbers below {shape[0]} of them, not at {kv.entry_offset}")
+    if kv.page_table.dtype != torch.int32 or kv.page_table.dim() != 2 or not kv.page_table.is_contiguous():
+        raise KernelError("page lists are a dense int32 tensor [n_seqs, pages]")
+
+
+def _quantised_rows(what: str, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor,
+                    kv: QuantisedKVView) -> tuple:
+    _check_quantised(kv, k, v, positions, tok_seq)
+    n = k.shape[0]
+    for t in (k, v):
+        if t is not None and (tuple(t.shape) != (n, kv.kv_heads, kv.head_dim) or t.dtype != k.dtype or (t.numel() and t.stride(2) != 1)):
+            raise KernelError(f"{what}: rows [tokens, {kv.kv_heads}, {kv.head_dim}] of one type with the head's numbers side by side, got "
+                              f"{tuple(t.shape)} {t.dtype} with strides {t.stride()}")
+    if v is None and kv.v_pool.data_ptr() != kv.k_pool.data_ptr():
+        raise KernelError(f"{what}: the entry has values of its own")
+    if v is not None and kv.v_pool.data_ptr() == kv.k_pool.data_ptr():
+        raise KernelError(f"{what}: the entry's values are its key rows; there are no others")
+    for t in (positions, tok_seq):
+        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+            raise KernelError(f"{what}: positions and sequences are dense int32, one per token")
+    vs = v if v is not None else k
+    return (k.data_ptr(), _ptr(v), dtype_code(k.dtype), k.stride(0), k.stride(1), vs.stride(0), vs.stride(1), positions.data_ptr(),
+            tok_seq.data_ptr(), n, kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+            kv.page_table.data_ptr(), kv.page_table.shape[0], kv.page_table.shape[1], kv.entry_offset, kv.k_pool.shape[1], kv.page_size,
+            kv.kv_heads, kv.head_dim, _stream())
+
+
+def quantise_kv(k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor, kv: QuantisedKVView) -> None:
+    """The rows k, v [tokens, kv_heads, head_dim] (float32 or bfloat16; token and head strides are free) into the cache, each
+    row's numbers in e4m3 beside the smallest power of two 2^e, -100 <= e <= 119, with max|x| <= 448 · 2^e (a larger row saturates; a row
+    with an infinity or a NaN reads as NaN).  Token i belongs at position positions[i] of sequence tok_seq[i]; one whose page is
+    missing is left out.  `v` is None for an entry whose values are its key rows."""
+    args = _quantised_rows("quantise_kv", k, v, positions, tok_seq, kv)
+    if k.shape[0]:
+        _check(core().mlc_quantise_kv(*args), "cache quantisation")
+
+
+def dequantise_kv(k_out: torch.Tensor, v_out: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor, kv: QuantisedKVView) -> None:
+    """The cached rows at the given places as numbers (exact in float32 and bfloat16), as `quantise_kv` takes them; zeros where
+    the page is missing."""
+    args = _quantised_rows("dequantise_kv", k_out, v_out, positions, tok_seq, kv)
+    if k_out.shape[0]:
+        _check(core().mlc_dequantise_kv(*args), "reading an 8-bit cache")
+
+
+_attn_q8_libs = {}
+
+
+def attention_q8_library(head_dim: int) -> ctypes.CDLL:
+    """The attention kernels over an 8-bit cache for one head size, built on first use."""
+    lib = _attn_q8_libs.get(head_dim)
+    if lib is None:
+        lib = _build.attention_q8_library(head_dim)
+        P, I, F, LL = c_void_p, c_int, c_float, c_longlong
+        lib.mlc_attention_q8.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
+        lib.mlc_attention_q8.restype = c_int
+        lib.mlc_attention_q8_head_dim.restype = c_int
+        if lib.mlc_attention_q8_head_dim() != head_dim:
+            raise KernelError(f"attention library built for head size {lib.mlc_attention_q8_head_dim()}, wanted {head_dim}")
+        _attn_q8_libs[head_dim] = lib
+    return lib
+
+
+def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, n_sms: int, window: int = 0,
+                      keep_first: int = 0, chunk: int = 0):
+    """(key_warps, n_splits, tiles_per_split) of the few-row form: 16 rows a block for single tokens and short chunks, else
+    64; tiles of 64 keys shared out in runs of one length, so that ragged batches come out even."""
+    group = q_heads // kv_heads
+    key_warps = 4 if max_q_len * min(group, 16) <= 32 else 1
+    rows = 16 if key_warps == 4 else 64
+    heads = min(group, rows)
+    tokens = rows // heads
+    blocks = ((max_q_len + tokens - 1) // tokens) * kv_heads * ((group + heads - 1) // heads) * n_seqs
+    tiles = (max_kv_len + 63) // 64
+    if window or chunk:             # a block's rows see the window of each of its tokens; an edge tile on either side
+        span = (chunk or window) + tokens + 126
+        tiles = min(tiles, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
+    wanted = max(1, (4 * n_sms + blocks - 1) // blocks)
+    per_split = max(4, (tiles + wanted - 1) // wanted)
+    n_splits = max(1, (tiles + per_split - 1) // per_split)
+    return key_warps, n_splits, per_split if n_splits > 1 else max(1, tiles)
+
+
+def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: torch.Tensor, n_seqs: int, max_q_len: int,
+                        max_kv_len: int, q_heads: int, kv: QuantisedKVView, scale: float, window: int = 0,
+                        sinks: Optional[torch.Tensor] = None, keep_first: int = 0, chunk: int = 0, softcap: float = 0.0) -> None:
+    """Attention of bfloat16 q [tokens, q_heads · head_dim] over an 8-bit cache entry, into `out` of the same shape: tokens
+    cu_seqlens[b] ... cu_seqlens[b + 1] are sequence b's, the first of them at position start_pos[b]; the entry holds their own keys already.
+    `max_q_len`, `max_kv_len`: bounds of a sequence's new tokens and of its keys with them.  `window`, `sinks`, `keep_first`, `chunk` and
+    `softcap` as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows behind the
+    last sequence's are left as they are."""
+    _check_quantised(kv, q, out, cu_seqlens, start_pos, sinks)
+    require_cuda(q, out, cu_seqlens, start_pos, sinks)
+    n = q.shape[0]
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise KernelError("attention over an 8-bit cache takes bfloat16 queries and output")
+    if q_heads <= 0 or q_heads % kv.kv_heads or q.numel() != n * q_heads * kv.head_dim or out.shape != q.shape:
+        raise KernelError(f"attention over an 8-bit cache: {q_heads} query heads on {kv.kv_heads} kv heads of {kv.head_dim}, q {tuple(q.shape)}, out {tuple(out.shape)}")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != q_heads):
+        raise KernelError("attention over an 8-bit cache: sinks are one float32 per query head")
+    for t, size in ((cu_seqlens, n_seqs + 1), (start_pos, n_seqs)):
+        if t.dtype != torch.int32 or t.numel() < size:
+            raise KernelError(f"attention over an 8-bit cache: sequence bounds are int32, {size} of them")
+    if kv.page_size != 64 or kv.page_table.shape[0] < n_seqs:
+        raise KernelError(f"attention over an 8-bit cache: pages of 64 tokens and a page list per sequence, got pages of {kv.page_size} and "
+                          f"{kv.page_table.shape[0]} lists for {n_seqs}")
+    if not scale > 0 or window < 0 or keep_first < 0 or chunk < 0 or not softcap >= 0 or (window and chunk):
+        raise KernelError(f"attention over an 8-bit cache: scale {scale}, window {window}, keep_first {keep_first}, chunk {chunk}, softcap {softcap}")
+    if n == 0 or n_seqs <= 0 or max_q_len <= 0:
+        return
+    lib = attention_q8_library(kv.head_dim)
+    key_warps, n_splits, per_split = attention_q8_plan(max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, _sm_count(q.device), window, keep_first, chunk)
+    part_ml = part_o = None
+    if n_splits > 1:
+        part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
+        part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
+    _check(lib.mlc_attention_q8(q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads,
+                                kv.kv_heads, kv.head_dim, float(scale), int(window), int(keep_first), int(chunk), float(softcap), _ptr(sinks),
+                                key_warps, n_splits, per_split, _ptr(part_ml), _ptr(part_o), kv.k_pool.data_ptr(), kv.v_pool.data_ptr(),
+                                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset,
+                                kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream()),
+           "attention over an 8-bit cache")
+    if n_splits > 1:
+        count_launches(1)

@@ -1,0 +1,291 @@
+"""Attention over the 8-bit cache against the definition in 64 bits, with bounds that count the roundings (plain_quantised.attention)."""
+import math
+
+import pytest
+import torch
+
+import plain_quantised as plain
+
+pytestmark = pytest.mark.gpu
+
+
+def kernels():
+    from mini_llama_cpp_release_b200 import kernels as k
+    return k
+
+
+class Case:
+    """Sequences (cached, new) over pages in no order; whatever no sequence's key owns is bytes of every kind, NaN codes and the scale of
+    a row that is not finite among them."""
+
+    def __init__(self, H, KV, hd, seqs, seed=0, entries=2, entry=1, shared=False, q_size=1.5, v_spread=0, k_rows=None, v_rows=None, tail=0):
+        dev = "cuda"
+        g = torch.Generator(device=dev).manual_seed(seed)
+        self.H, self.KV, self.hd, self.seqs = H, KV, hd, seqs
+        lens = [c + n for c, n in seqs]
+        n_pages = sum((t + 63) // 64 for t in lens) + 2
+        width = max(1, max((t + 63) // 64 for t in lens))
+        order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        self.table = torch.full((len(seqs), width), -1, dtype=torch.int32)
+        shape = (entries, n_pages, KV, 64, hd)
+        self.codes = [torch.randint(0, 256, shape, generator=g, device=dev).to(torch.uint8) for _ in range(1 if shared else 2)]
+        self.scales = [torch.randint(0, 256, shape[:4], generator=g, device=dev).to(torch.uint8) for _ in range(1 if shared else 2)]
+        for t in self.codes:
+            t[:, :, :, ::5] = 0x7f
+        for t in self.scales:
+            t[:, :, :, ::7] = 255
+        self.k, self.v = [], []
+        for b, t in enumerate(lens):
+            pages = [order.pop() for _ in range((t + 63) // 64)]
+            self.table[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+            k = torch.randn(t, KV, hd, generator=g, device=dev) if k_rows is None else k_rows(b, t, g)
+            v = torch.randn(t, KV, hd, generator=g, device=dev) if v_rows is None else v_rows(b, t, g)
+            if v_spread:
+                v = v * torch.exp2(torch.randint(-v_spread, v_spread + 1, (t, KV, 1), generator=g, device=dev).float())
+            kept = []
+            for i, x in enumerate((k,) if shared else (k, v)):
+                codes, byte = plain.quantise(x)
+                kept.append(plain.values(codes, byte))
+                for p, page in enumerate(pages):
+                    n = min(64, t - 64 * p)
+                    self.codes[i][entry, page, :, :n] = codes[64 * p:64 * p + n].transpose(0, 1)
+                    self.scales[i][entry, page, :, :n] = byte[64 * p:64 * p + n].T
+            self.k.append(kept[0])
+            self.v.append(kept[-1])
+        self.n = sum(n for _, n in seqs)
+        self.tail = tail
+        self.q = (torch.randn(self.n + tail, H * hd, generator=g, device=dev) * q_size).bfloat16()
+        self.cu = torch.tensor([0] + [n for _, n in seqs]).cumsum(0).int().to(dev)
+        self.start = torch.tensor([c for c, _ in seqs], dtype=torch.int32, device=dev)
+        self.sinks = torch.randn(H, generator=g, device=dev)
+        self.entry, self.shared = entry, shared
+
+    def view(self, table=None):
+        e4 = torch.float8_e4m3fn
+        k, ks = self.codes[0].view(e4), self.scales[0]
+        v, vs = (k, ks) if self.shared else (self.codes[1].view(e4), self.scales[1])
+        return kernels().QuantisedKVView(k, v, ks, vs, self.entry * self.codes[0][0].numel(), (self.table if table is None else table).cuda(), 64,
+                                         self.KV, self.hd)
+
+    def run(self, scale=None, window=0, keep_first=0, chunk=0, softcap=0.0, sinks=False, table=None, out=None, max_kv=None):
+        out = torch.full_like(self.q, 7.0) if out is None else out
+        kernels().attention_quantised(self.q, out, self.cu, self.start, len(self.seqs), max(n for _, n in self.seqs),
+                                      max(c + n for c, n in self.seqs) if max_kv is None else max_kv, self.H, self.view(table),
+                                      self.hd ** -0.5 if scale is None else scale, window, sinks=self.sinks if sinks else None,
+                                      keep_first=keep_first, chunk=chunk, softcap=softcap)
+        return out
+
+    def check(self, out, scale=None, window=0, keep_first=0, chunk=0, softcap=0.0, sinks=False, gone=()):
+        """`gone`: (sequence, page index) whose page is missing."""
+        at = 0
+        for b, (c, n) in enumerate(self.seqs):
+            if n == 0:
+                continue
+            seen = plain.visible(torch.arange(c, c + n, device="cuda"), c + n, window, keep_first, chunk)
+            for s, p in gone:
+                if s == b:
+                    seen[:, 64 * p:64 * p + 64] = False
+            q = self.q[at:at + n].view(n, self.H, self.hd)
+            want, bound = plain.attention(q, self.k[b], self.v[b], seen, self.hd ** -0.5 if scale is None else scale,
+                                          self.sinks if sinks else None, softcap)
+            got = out[at:at + n].view(n, self.H, self.hd).double()
+            assert torch.isfinite(got).all(), f"sequence {b}"
+            worst = ((got - want).abs() / bound).max()
+            assert worst <= 1.0, f"sequence {b}: {float(worst):.3g} of the bound"
+            at += n
+        if self.tail:
+            assert (out[self.n:] == 7.0).all(), "rows behind the last sequence"
+        kernels().check_gemm_status(torch.device("cuda", 0))
+
+
+LAYOUTS = [(14, 2, 64), (12, 2, 128), (4, 4, 16), (6, 2, 48), (8, 1, 256), (40, 2, 64)]
+SINGLES = [
+    [(0, 1)],
+    [(62, 1)], [(63, 1)], [(64, 1)],
+    [(0, 1), (1, 1), (64, 1), (999, 1), (127, 1)],
+    [(5000, 1), (3, 1)],
+]
+
+
+@pytest.mark.parametrize("H,KV,hd", LAYOUTS)
+@pytest.mark.parametrize("seqs", SINGLES, ids=[str(i) for i in range(len(SINGLES))])
+def test_single_tokens(H, KV, hd, seqs):
+    c = Case(H, KV, hd, seqs, tail=2)
+    c.check(c.run())
+
+
+MASKS = [
+    dict(window=1), dict(window=64), dict(window=100, keep_first=4), dict(window=3, keep_first=130), dict(window=2000, keep_first=1),
+    dict(chunk=1), dict(chunk=100), dict(softcap=5.0), dict(sinks=True), dict(window=70, keep_first=65, sinks=True, softcap=3.0),
+]
+
+
+@pytest.mark.parametrize("mask", MASKS, ids=[str(m) for m in MASKS])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (6, 2, 48)])
+def test_single_tokens_with_masks(H, KV, hd, mask):
+    c = Case(H, KV, hd, [(700, 1), (0, 1), (99, 1), (100, 1), (63, 1), (1500, 1)], seed=3)
+    c.check(c.run(**mask), **mask)
+
+
+CHUNKS = [
+    [(0, 2)],
+    [(0, 64)], [(0, 65)], [(63, 2), (0, 1), (64, 64)],
+    [(300, 129), (0, 1), (1000, 17), (5, 300)],
+    [(0, 700), (2500, 90)],
+]
+
+
+@pytest.mark.parametrize("H,KV,hd", LAYOUTS)
+@pytest.mark.parametrize("seqs", CHUNKS, ids=[str(i) for i in range(len(CHUNKS))])
+def test_chunks(H, KV, hd, seqs):
+    c = Case(H, KV, hd, seqs, seed=1, tail=3)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("mask", MASKS, ids=[str(m) for m in MASKS])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (6, 2, 48)])
+def test_chunks_with_masks(H, KV, hd, mask):
+    c = Case(H, KV, hd, [(700, 150), (0, 1), (0, 260), (100, 5), (1500, 40)], seed=4)
+    c.check(c.run(**mask), **mask)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs", [[(4000, 1)], [(800, 200)]], ids=["single", "chunk"])
+def test_values_whose_rows_differ_by_many_binades(hd, seqs):
+    c = Case(14, 2, hd, seqs, seed=5, v_spread=20)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("seqs", [[(900, 1)], [(300, 200)]], ids=["single", "chunk"])
+def test_values_of_zeros_count_in_the_denominator(seqs):
+    """Rows of zeros have the lowest scale; rows far larger than the others must not push them out of the sum."""
+    def rows(b, t, g):
+        v = torch.zeros(t, 2, 64, device="cuda")
+        v[::50] = 2.0 ** 22 * torch.randn(v[::50].shape, generator=g, device="cuda")
+        return v
+    c = Case(14, 2, 64, seqs, seed=6, v_rows=rows)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("seqs", [[(500, 1), (20, 1)], [(300, 200)]], ids=["single", "chunk"])
+def test_values_read_out_of_the_key_rows(seqs):
+    c = Case(14, 1, 128, seqs, seed=7, shared=True)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("exponent", [-60, 60])
+@pytest.mark.parametrize("seqs", [[(500, 1)], [(300, 200)]], ids=["single", "chunk"])
+def test_large_queries_on_small_keys(exponent, seqs):
+    def rows(b, t, g):
+        return torch.randn(t, 2, 64, generator=g, device="cuda") * 2.0 ** -exponent
+    c = Case(14, 2, 64, seqs, seed=8, q_size=2.0 ** exponent, k_rows=rows)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("seqs", [[(900, 1), (64, 1)], [(300, 200), (0, 70)]], ids=["single", "chunk"])
+@pytest.mark.parametrize("value", [-1, 10 ** 6], ids=["negative", "beyond the pool"])
+def test_missing_pages(seqs, value):
+    c = Case(14, 2, 64, seqs, seed=9)
+    table = c.table.clone()
+    table[0, 2] = value
+    table[1, 0] = value
+    c.check(c.run(table=table), gone=[(0, 2), (1, 0)])
+
+
+@pytest.mark.parametrize("seqs", [[(30, 1), (100, 1)], [(0, 40), (60, 130)]], ids=["single", "chunk"])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_rows_that_see_no_key_are_zeros(seqs, sinks):
+    c = Case(14, 2, 64, seqs, seed=10)
+    table = c.table.clone()
+    table[0, :] = -1
+    out = c.run(table=table, sinks=sinks)
+    assert not out[:seqs[0][1]].any()
+    c.check(out, gone=[(0, p) for p in range(c.table.shape[1])], sinks=sinks)
+
+
+@pytest.mark.parametrize("seqs,window", [([(200, 1), (200, 1)], 100), ([(130, 100), (130, 100)], 50)], ids=["single", "chunk"])
+@pytest.mark.parametrize("which", [0, 1], ids=["keys", "values"])
+def test_a_row_that_is_not_finite_reaches_those_that_see_it_only(seqs, window, which):
+    c = Case(14, 2, 64, seqs, seed=11)
+    clean = c.run(window=window)
+    spoilt = 140                                   # of sequence 0, kv head 1
+    c.codes[which][1, c.table[0, spoilt // 64], 1, spoilt % 64] = 0
+    c.scales[which][1, c.table[0, spoilt // 64], 1, spoilt % 64] = 255
+    out = c.run(window=window).view(-1, 14, 64)
+    clean = clean.view(-1, 14, 64)
+    n = seqs[0][1]
+    p = torch.arange(seqs[0][0], seqs[0][0] + n, device="cuda")
+    sees = (spoilt <= p) & (p - spoilt < window)
+    hit = torch.zeros(out.shape[0], 14, dtype=torch.bool, device="cuda")
+    hit[:n, 7:] = sees[:, None]
+    assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
+
+
+def test_a_window_whose_pages_were_given_back():
+    c = Case(14, 2, 64, [(1000, 1), (900, 30)], seed=12)
+    table = c.table.clone()
+    for b, first in ((0, 1000 - 100 + 1), (1, 900 - 100 + 1)):
+        table[b, 1:first // 64] = -1
+    c.check(c.run(window=100, keep_first=4, table=table), window=100, keep_first=4)
+
+
+def test_empty_sequences_and_bounds_that_are_too_large_or_too_small():
+    c = Case(14, 2, 64, [(10, 0), (200, 3), (0, 0), (64, 1), (5, 0)], seed=13, tail=1)
+    c.check(c.run())
+    c.check(c.run(max_kv=30000))
+    c.check(c.run(max_kv=1))                       # a bound that is too small costs time, not keys
+
+
+@pytest.mark.parametrize("seqs", [[(2000, 1)] * 3, [(500, 100), (0, 300)]], ids=["single", "chunk"])
+def test_captured_on_another_stream_and_two_graphs_at_once(seqs):
+    a, b = Case(14, 2, 64, seqs, seed=14), Case(14, 2, 64, seqs, seed=15)
+    outs = [torch.zeros_like(a.q), torch.zeros_like(b.q)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    views = [a.view(), b.view()]
+    graphs = []
+
+    def call(i):
+        c = (a, b)[i]
+        kernels().attention_quantised(c.q, outs[i], c.cu, c.start, len(seqs), max(n for _, n in seqs), max(x + n for x, n in seqs), 14, views[i], 0.125)
+
+    for i in range(2):
+        streams[i].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[i]):
+            call(i)
+        streams[i].synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            call(i)
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        a.check(outs[0])
+        b.check(outs[1])
+
+
+def test_the_same_call_twice_gives_the_same_bits():
+    for seqs in ([(3000, 1), (17, 1)], [(300, 200)]):
+        c = Case(14, 2, 64, seqs, seed=16)
+        assert torch.equal(c.run(), c.run())
+
+
+def test_refusals():
+    import dataclasses
+    K = kernels()
+    c = Case(14, 2, 64, [(10, 1)], seed=17)
+    kv = c.view()
+    ok = dict(q=c.q, out=torch.empty_like(c.q), cu=c.cu, start=c.start, n_seqs=1, H=14, kv=kv, scale=0.1, more={})
+    bad = [dict(q=c.q.float()), dict(out=c.q.float()), dict(H=13), dict(H=28), dict(n_seqs=2), dict(cu=c.cu.long()), dict(scale=0.0), dict(scale=math.nan),
+           dict(more=dict(window=-1)), dict(more=dict(window=4, chunk=4)), dict(more=dict(softcap=-1.0)), dict(more=dict(softcap=math.nan)),
+           dict(more=dict(keep_first=-1)), dict(more=dict(sinks=c.sinks[:3])), dict(more=dict(sinks=c.sinks.double())),
+           dict(kv=dataclasses.replace(kv, page_size=32)), dict(q=c.q.cpu()), dict(out=torch.empty(1, 14 * 64 * 2, device="cuda", dtype=torch.bfloat16)[:, ::2])]
+    for change in bad:
+        a = {**ok, **change}
+        with pytest.raises(K.KernelError):
+            K.attention_quantised(a["q"], a["out"], a["cu"], a["start"], a["n_seqs"], 1, 11, a["H"], a["kv"], a["scale"], **a["more"])
