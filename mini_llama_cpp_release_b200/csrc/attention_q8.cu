@@ -507,6 +507,16 @@ static cudaError_t shared_memory_of(const void* kernel, int bytes, int which) {
 
 extern "C" int mlc_attention_q8_head_dim() { return Q_HD; }
 
+// Joins n_splits partial results a row (layouts: Q8Args).
+extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_o, const int* cu_seqlens, int n_seqs, int n_tokens, int q_heads,
+                                        int n_splits, const float* sinks, void* out, void* stream) {
+    const long long blocks = ((long long)n_tokens * q_heads + 3) / 4;
+    if (blocks > 0x7fffffffll) return MLC_ERR_BAD_SIZE;
+    const cudaError_t e = launch_pdl(q8_combine_kernel, dim3((unsigned)blocks), dim3(128), (size_t)0, (cudaStream_t)stream, part_ml, part_o, cu_seqlens,
+                                     n_seqs, n_tokens, q_heads, n_splits, sinks, (bf16*)out);
+    return e == cudaSuccess ? 0 : (int)e;
+}
+
 // q, out: bfloat16 [n_tokens][q_heads · head_dim], 16-byte aligned.  The entry starts `entry_offset` codes into the pools, which hold
 // `n_pages` pages of 64 tokens an entry.  key_warps: 4 (16 rows a block) or 1 (64 rows).  tiles_per_split: tiles of 64 keys a block
 // walks (the last of the n_splits goes on to the end); more than one need part_ml (n_tokens · q_heads · n_splits · 2 floats) and part_o
@@ -558,10 +568,6 @@ extern "C" int mlc_attention_q8(const void* q, void* out, const int* cu_seqlens,
     if (e != cudaSuccess) return (int)e;
     cudaStream_t s = (cudaStream_t)stream;
     e = launch_pdl(kernel, dim3((unsigned)blocks, n_seqs), dim3(Q_THREADS), (size_t)Q_SMEM_BYTES, s, a);
-    if (e != cudaSuccess || n_splits == 1) return e == cudaSuccess ? 0 : (int)e;
-    const long long out_rows = (long long)n_tokens * q_heads;
-    if ((out_rows + 3) / 4 > 0x7fffffffll) return MLC_ERR_BAD_SIZE;
-    e = launch_pdl(q8_combine_kernel, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), (size_t)0, s, (const float*)part_ml, (const float*)part_o, cu_seqlens, n_seqs,
-                   n_tokens, q_heads, n_splits, sinks, (bf16*)out);
-    return e == cudaSuccess ? 0 : (int)e;
+    if (e != cudaSuccess) return (int)e;
+    return n_splits == 1 ? 0 : mlc_attention_q8_combine(part_ml, part_o, cu_seqlens, n_seqs, n_tokens, q_heads, n_splits, sinks, out, stream);
 }

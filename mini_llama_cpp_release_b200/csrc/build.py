@@ -37,7 +37,7 @@ CORE_SOURCES = ["elementwise.cu", "attention_simt.cu", "sampling.cu", "linear_si
 # compiled once per head size (-DMLC_HEAD_DIM=...): the mma.sync kernels for every size, the tcgen05 kernel for 64 and 128
 ATTENTION_SOURCES = ["attention_mma.cu", "attention_tcgen05.cu"]
 # the same over an 8-bit cache, built when a cache of that kind is asked for
-ATTENTION_Q8_SOURCES = ["attention_q8.cu"]
+ATTENTION_Q8_SOURCES = ["attention_q8.cu", "attention_q8_tcgen05.cu"]
 
 _lock = threading.Lock()
 _loaded: Dict[str, ctypes.CDLL] = {}

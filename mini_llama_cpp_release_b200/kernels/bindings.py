@@ -22,7 +22,7 @@ __all__ = [
     "group_norm", "activation", "forget_gate_attention", "moe_route_scored",
     "tanh_norm", "glu", "sigmoid_gate", "state_space",
     "decay_attention", "matrix_memory", "rms_pair", "embed_rms", "diff_combine", "moe_plan_table",
-    "QuantisedKVView", "quantise_kv", "dequantise_kv", "attention_quantised", "attention_q8_library", "attention_q8_plan",
+    "QuantisedKVView", "quantise_kv", "dequantise_kv", "attention_quantised", "attention_q8_library", "attention_q8_plan", "attention_q8_tcgen05_plan",
 ]
 
 
@@ -1351,7 +1351,9 @@ def check_gemm_status(device: torch.device) -> None:
                    23: "the prompt product's epilogue", 31: "the single-token attention kernel's wait for keys and values", 41: "the paired prompt product's TMA loader",
                    42: "the paired prompt product's tensor-core issuer or relay", 43: "the paired prompt product's epilogue",
                    61: "the float32 few-row product's wait for its operands", 71: "the 8-bit cache attention's loader",
-                   72: "the 8-bit cache attention's wait for keys and values"}.get(code, str(code))
+                   72: "the 8-bit cache attention's wait for keys and values",
+                   73: "the 8-bit cache prompt attention's loader", 74: "the 8-bit cache prompt attention's score issuer",
+                   75: "the 8-bit cache prompt attention's output issuer", 76: "the 8-bit cache prompt attention's rows or converters"}.get(code, str(code))
             raise KernelError(f"a tcgen05 kernel gave up waiting on a barrier ({who}); its output is not valid")
 
 
@@ -1879,6 +1881,8 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
         P, I, F, LL = c_void_p, c_int, c_float, c_longlong
         lib.mlc_attention_q8.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
         lib.mlc_attention_q8.restype = c_int
+        lib.mlc_attention_q8_tcgen05.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
+        lib.mlc_attention_q8_tcgen05.restype = c_int
         lib.mlc_attention_q8_head_dim.restype = c_int
         if lib.mlc_attention_q8_head_dim() != head_dim:
             raise KernelError(f"attention library built for head size {lib.mlc_attention_q8_head_dim()}, wanted {head_dim}")
@@ -1904,6 +1908,26 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
     per_split = max(4, (tiles + wanted - 1) // wanted)
     n_splits = max(1, (tiles + per_split - 1) // per_split)
     return key_warps, n_splits, per_split if n_splits > 1 else max(1, tiles)
+
+
+def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
+                              keep_first: int = 0, chunk: int = 0):
+    """(n_splits, tiles_per_split) of the form with 256 rows a block, or None where it is not for these sizes."""
+    group = q_heads // kv_heads
+    if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len * group < 64:
+        return None
+    heads = min(group, 128)
+    tokens = 2 * (128 // heads)
+    blocks = ((max_q_len + tokens - 1) // tokens) * kv_heads * ((group + heads - 1) // heads) * n_seqs
+    longest = (max_kv_len + 63) // 64
+    if window or chunk:
+        span = (chunk or window) + tokens + 126
+        longest = min(longest, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
+    if blocks >= 3 * n_sms:
+        return 1, longest
+    per_split = max(8, blocks * longest // (3 * n_sms))
+    n_splits = (longest + per_split - 1) // per_split
+    return n_splits, per_split
 
 
 def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: torch.Tensor, n_seqs: int, max_q_len: int,
@@ -1934,16 +1958,21 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     if n == 0 or n_seqs <= 0 or max_q_len <= 0:
         return
     lib = attention_q8_library(kv.head_dim)
-    key_warps, n_splits, per_split = attention_q8_plan(max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, _sm_count(q.device), window, keep_first, chunk)
+    sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads)
+    prompt = attention_q8_tcgen05_plan(*sizes, kv.head_dim, _sm_count(q.device), window, keep_first, chunk)
+    if prompt is not None:
+        n_splits, per_split = prompt
+    else:
+        key_warps, n_splits, per_split = attention_q8_plan(*sizes, _sm_count(q.device), window, keep_first, chunk)
     part_ml = part_o = None
     if n_splits > 1:
         part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
         part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
-    _check(lib.mlc_attention_q8(q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads,
-                                kv.kv_heads, kv.head_dim, float(scale), int(window), int(keep_first), int(chunk), float(softcap), _ptr(sinks),
-                                key_warps, n_splits, per_split, _ptr(part_ml), _ptr(part_o), kv.k_pool.data_ptr(), kv.v_pool.data_ptr(),
-                                kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset,
-                                kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream()),
-           "attention over an 8-bit cache")
+    head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, float(scale),
+            int(window), int(keep_first), int(chunk), float(softcap), _ptr(sinks))
+    tail = (n_splits, per_split, _ptr(part_ml), _ptr(part_o), kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+            kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset, kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream())
+    rc = lib.mlc_attention_q8_tcgen05(*head, *tail) if prompt is not None else lib.mlc_attention_q8(*head, key_warps, *tail)
+    _check(rc, "attention over an 8-bit cache")
     if n_splits > 1:
         count_launches(1)
