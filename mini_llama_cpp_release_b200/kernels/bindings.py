@@ -1881,7 +1881,7 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
         P, I, F, LL = c_void_p, c_int, c_float, c_longlong
         lib.mlc_attention_q8.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
         lib.mlc_attention_q8.restype = c_int
-        lib.mlc_attention_q8_tcgen05.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
+        lib.mlc_attention_q8_tcgen05.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, P, P, P, I, P, P, P, P, P, I, LL, LL, I, P, P]
         lib.mlc_attention_q8_tcgen05.restype = c_int
         lib.mlc_attention_q8_head_dim.restype = c_int
         if lib.mlc_attention_q8_head_dim() != head_dim:
@@ -1910,24 +1910,37 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
     return key_warps, n_splits, per_split if n_splits > 1 else max(1, tiles)
 
 
+EXPANDED_BYTES = 8 << 30        # the most scratch memory for pages written out as bfloat16 (a call that would want more runs in the form without)
+
+
+def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
+    """n bfloat16 numbers of scratch memory; None where that is too much or there is no room for it."""
+    if 2 * n > EXPANDED_BYTES:
+        return None
+    try:
+        return torch.empty(n, dtype=torch.bfloat16, device=device)
+    except torch.OutOfMemoryError:
+        return None
+
+
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
-    """(n_splits, tiles_per_split) of the form with 256 rows a block, or None where it is not for these sizes."""
+    """(n_splits, tiles_per_split) of the form with 128 rows a block, or None where it is not for these sizes."""
     group = q_heads // kv_heads
     if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len * group < 64:
         return None
     heads = min(group, 128)
-    tokens = 2 * (128 // heads)
+    tokens = 128 // heads
     blocks = ((max_q_len + tokens - 1) // tokens) * kv_heads * ((group + heads - 1) // heads) * n_seqs
     longest = (max_kv_len + 63) // 64
     if window or chunk:
         span = (chunk or window) + tokens + 126
         longest = min(longest, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
-    if blocks >= 3 * n_sms:
-        return 1, longest
-    per_split = max(8, blocks * longest // (3 * n_sms))
-    n_splits = (longest + per_split - 1) // per_split
-    return n_splits, per_split
+    # a key range is shared out only to fill the first wave of blocks: the joining costs what it saves from there on (one prompt of 4,095 tokens, 14 heads
+    # of 64 on 2, 228 blocks: 55 us, in two splits 83)
+    wanted = max(1, n_sms // blocks)
+    per_split = max(8, (longest + wanted - 1) // wanted)
+    return (longest + per_split - 1) // per_split, per_split
 
 
 def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: torch.Tensor, n_seqs: int, max_q_len: int,
@@ -1960,7 +1973,12 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     lib = attention_q8_library(kv.head_dim)
     sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads)
     prompt = attention_q8_tcgen05_plan(*sizes, kv.head_dim, _sm_count(q.device), window, keep_first, chunk)
+    dense = None
     if prompt is not None:
+        # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
+        dense_tiles = max(1, kv.pages_per_seq)
+        dense = _spare_rows(n_seqs * kv.kv_heads * dense_tiles * 128 * kv.head_dim, q.device)
+    if dense is not None:
         n_splits, per_split = prompt
     else:
         key_warps, n_splits, per_split = attention_q8_plan(*sizes, _sm_count(q.device), window, keep_first, chunk)
@@ -1970,9 +1988,14 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
         part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
     head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, float(scale),
             int(window), int(keep_first), int(chunk), float(softcap), _ptr(sinks))
-    tail = (n_splits, per_split, _ptr(part_ml), _ptr(part_o), kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
-            kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset, kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream())
-    rc = lib.mlc_attention_q8_tcgen05(*head, *tail) if prompt is not None else lib.mlc_attention_q8(*head, key_warps, *tail)
+    parts = (n_splits, per_split, _ptr(part_ml), _ptr(part_o))
+    tail = (kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset,
+            kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream())
+    if dense is not None:
+        rc = lib.mlc_attention_q8_tcgen05(*head, *parts, dense.data_ptr(), dense_tiles, *tail)
+        count_launches(1)
+    else:
+        rc = lib.mlc_attention_q8(*head, key_warps, *parts, *tail)
     _check(rc, "attention over an 8-bit cache")
     if n_splits > 1:
         count_launches(1)
