@@ -1890,26 +1890,32 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     return lib
 
 
-def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, n_sms: int, window: int = 0,
+def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                       keep_first: int = 0, chunk: int = 0):
-    """(key_warps, n_splits, tiles_per_split) of the few-row form: 16 rows a block for single tokens and short chunks, else
-    64; tiles of 64 keys shared out in runs of one length, so that ragged batches come out even."""
+    """(rows, n_splits, tiles_per_split, in_cluster) of the form without scratch pages: 8, 16 or 64 rows a block, tiles of 64 keys shared out
+    in runs of one length.  Splits fill one wave of blocks, a tile for each of a block's four warps at least; where the rows alone fill it, runs of 32 tiles even out
+    ragged batches (64 sequences of up to 8,191 keys, 28 heads of 128 on 4: 57 us, whole sequences 85).  Up to eight splits of one wave join inside a cluster (one
+    sequence of 2,000 keys, 14 heads of 64 on 2: 6.2 us, with a second kernel 7.0; in more waves a cluster waits for its longest split: 82 us for the 57)."""
     group = q_heads // kv_heads
-    key_warps = 4 if max_q_len * min(group, 16) <= 32 else 1
-    rows = 16 if key_warps == 4 else 64
+    few = max_q_len * group
+    rows = 8 if few <= 8 else 16 if few <= 32 else 64
     heads = min(group, rows)
     tokens = rows // heads
     blocks = ((max_q_len + tokens - 1) // tokens) * kv_heads * ((group + heads - 1) // heads) * n_seqs
-    tiles = (max_kv_len + 63) // 64
+    tiles = max(1, (max_kv_len + 63) // 64)
     if window or chunk:             # a block's rows see the window of each of its tokens; an edge tile on either side
         span = (chunk or window) + tokens + 126
         tiles = min(tiles, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
-    wanted = max(1, (4 * n_sms + blocks - 1) // blocks)
-    per_split = max(4, (tiles + wanted - 1) // wanted)
-    n_splits = max(1, (tiles + per_split - 1) // per_split)
-    return key_warps, n_splits, per_split if n_splits > 1 else max(1, tiles)
+    wave = n_sms * (3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) // (1 if rows == 8 else 2)
+    splits = wave // blocks
+    per_split = max(4, (-(-tiles // splits) + 3) // 4 * 4) if splits > 1 else 32
+    if tiles < 1.5 * per_split:
+        return rows, 1, tiles, False
+    n_splits = -(-tiles // per_split)
+    return rows, n_splits, per_split, rows != 64 and n_splits <= Q8_CLUSTER and blocks * n_splits <= wave
 
 
+Q8_CLUSTER = 8                  # the most key splits that join inside a thread-block cluster, without scratch memory and a second kernel
 EXPANDED_BYTES = 8 << 30        # the most scratch memory for pages written out as bfloat16 (a call that would want more runs in the form without)
 
 
@@ -1971,9 +1977,9 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     if n == 0 or n_seqs <= 0 or max_q_len <= 0:
         return
     lib = attention_q8_library(kv.head_dim)
-    sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads)
-    prompt = attention_q8_tcgen05_plan(*sizes, kv.head_dim, _sm_count(q.device), window, keep_first, chunk)
-    dense = None
+    sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, kv.head_dim, _sm_count(q.device), window, keep_first, chunk)
+    prompt = attention_q8_tcgen05_plan(*sizes)
+    dense, in_cluster = None, False
     if prompt is not None:
         # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
         dense_tiles = max(1, kv.pages_per_seq)
@@ -1981,9 +1987,10 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     if dense is not None:
         n_splits, per_split = prompt
     else:
-        key_warps, n_splits, per_split = attention_q8_plan(*sizes, _sm_count(q.device), window, keep_first, chunk)
+        rows, n_splits, per_split, in_cluster = attention_q8_plan(*sizes)
     part_ml = part_o = None
-    if n_splits > 1:
+    joined_later = n_splits > 1 and not in_cluster
+    if joined_later:
         part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
         part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
     head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, float(scale),
@@ -1995,7 +2002,7 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
         rc = lib.mlc_attention_q8_tcgen05(*head, *parts, dense.data_ptr(), dense_tiles, *tail)
         count_launches(1)
     else:
-        rc = lib.mlc_attention_q8(*head, key_warps, *parts, *tail)
+        rc = lib.mlc_attention_q8(*head, rows, *parts, *tail)
     _check(rc, "attention over an 8-bit cache")
-    if n_splits > 1:
+    if joined_later:
         count_launches(1)
