@@ -19,10 +19,10 @@ from .sampling.sampler import DeviceSampler, SamplingParams
 
 class LLM:
     def __init__(self, model: Model, max_tokens: int, max_seqs: Optional[int] = None,
-                 max_batch_tokens: int = EngineConfig.max_batch_tokens):
+                 max_batch_tokens: int = EngineConfig.max_batch_tokens, cache_dtype=None):
         self.model = model
         self.config = model.config
-        self.context = Context(model, max_tokens, max_seqs, max_batch_tokens=max_batch_tokens)
+        self.context = Context(model, max_tokens, max_seqs, max_batch_tokens=max_batch_tokens, cache_dtype=cache_dtype)
 
     def generate(self, prompts: Sequence[Sequence[int]], n_predict: Union[int, Sequence[int]] = 16, temperature: float = 0.0,
                  top_k: int = 0, seed: int = 0, stop_token_ids: Optional[Sequence[int]] = None,
@@ -43,19 +43,20 @@ class LLM:
 
 def load(folder: str, dtype="bfloat16", device: str = "cuda:0", max_tokens: int = 8192,
          max_seqs: Optional[int] = None, max_batch_tokens: Optional[int] = None, engine: Optional[EngineConfig] = None,
-         config_path: Optional[str] = None) -> LLM:
+         config_path: Optional[str] = None, cache_dtype=None) -> LLM:
     """A model folder (config.json + model.safetensors) → an `LLM` on a CUDA device.  How it runs is an `EngineConfig`,
     given whole as `engine` or by its fields as keywords: `max_tokens` sizes the cache (the most tokens live sequences
-    hold at any time, each rounded up to 64), `max_seqs` the number of slots, `max_batch_tokens` the largest step.
+    hold at any time, each rounded up to 64), `max_seqs` the number of slots, `max_batch_tokens` the largest step, `cache_dtype="float8_e4m3"` keeps
+    keys and values in 8 bits.
     `folder` may also be the path of one .safetensors file; its config.json is then `config_path`, or lies beside it."""
     if engine is None:
-        engine = EngineConfig(dtype=dtype, device=device, max_tokens=max_tokens, max_seqs=max_seqs,
+        engine = EngineConfig(dtype=dtype, device=device, max_tokens=max_tokens, max_seqs=max_seqs, cache_dtype=cache_dtype,
                               **({} if max_batch_tokens is None else {"max_batch_tokens": max_batch_tokens}))
     # float32 products must be float32: no TF32, no reduced-precision accumulation
     torch.backends.cuda.matmul.allow_tf32 = False
     torch.backends.cudnn.allow_tf32 = False
     torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
     model = Model.from_folder(folder, engine.dtype, engine.device, config_path=config_path)
-    llm = LLM(model, engine.max_tokens, engine.max_seqs, engine.max_batch_tokens)
+    llm = LLM(model, engine.max_tokens, engine.max_seqs, engine.max_batch_tokens, engine.cache_dtype)
     llm.engine = engine
     return llm

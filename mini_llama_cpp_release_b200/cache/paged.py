@@ -8,6 +8,10 @@ so the keys of one (page, kv head) are one dense block.  The reference's cache i
 (src/kv_cache.cpp:14-17, 41-45); nothing is zero-filled here because reads stop at each
 sequence's own length.
 
+With an element type of float8_e4m3fn the pools hold 8-bit numbers, and beside each pool lie the scale bytes of its rows,
+[entries of the group][pages][kv_heads][page_size] (csrc/quantised.cuh says what they mean): head_dim + 1 bytes a row.  Page lists,
+groups and windows are the same.
+
 A *group* collects the schedule entries whose mixers declared the same need (all keys,
 or a window of them, with the same heads and head size); each group has its own pools,
 its own free list and its own page lists, so a model whose layers need different things
@@ -21,11 +25,12 @@ declares none; the area exists so that a mixer that needs it finds it.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ..kernels import KVView
+from .. import kernels
+from ..kernels import KVView, QuantisedKVView
 from ..parts.base import CacheNeed, StateSpec
 from .pool import CacheFull, CacheMisuse, FreeList
 
@@ -81,11 +86,16 @@ def plan_groups(needs: Sequence[Optional[CacheNeed]], reads_cache_of: Sequence[O
     return groups, where
 
 
+def _row_bytes(need: CacheNeed, itemsize: int, scales: int = 0) -> int:
+    """Bytes of one token's keys and values in one entry: numbers of `itemsize` bytes and `scales` bytes a row."""
+    return (1 if need.shared_kv else 2) * need.kv_heads * (need.head_dim * itemsize + scales)
+
+
 def cache_bytes_per_token(needs: Sequence[Optional[CacheNeed]], reads_cache_of: Sequence[Optional[int]], itemsize: int) -> int:
     """Key and value bytes one token of one sequence occupies over all groups, for elements of `itemsize` bytes
     (a window group holds at most its window of them)."""
     groups, _ = plan_groups(needs, reads_cache_of)
-    return sum((1 if g.need.shared_kv else 2) * len(g.entries) * g.need.kv_heads * g.need.head_dim * itemsize for g in groups)
+    return sum(len(g.entries) * _row_bytes(g.need, itemsize) for g in groups)
 
 
 class SlotBook:
@@ -218,13 +228,24 @@ class PagedCache(SlotBook):
         self.where = where
         self.dtype = dtype
         self.device = device
+        self.quantised = dtype == torch.float8_e4m3fn
+        if self.quantised:
+            for layout in groups:
+                if layout.need.head_dim % 16 or layout.need.head_dim > 256 or page_size != 64:
+                    raise ValueError(f"an 8-bit cache takes heads of 16, 32, ..., 256 numbers and pages of 64 tokens, not heads of "
+                                     f"{layout.need.head_dim} and pages of {page_size}")
         self.k_pools: List[torch.Tensor] = []
         self.v_pools: List[torch.Tensor] = []
+        self.k_scales: List[Optional[torch.Tensor]] = []           # of an 8-bit cache
+        self.v_scales: List[Optional[torch.Tensor]] = []
         for layout in groups:
             shape = (len(layout.entries), self.n_pages, layout.need.kv_heads, page_size, layout.need.head_dim)
             self.k_pools.append(torch.empty(shape, dtype=dtype, device=device))
             # a group whose values are read out of its key rows has one pool under both names
             self.v_pools.append(self.k_pools[-1] if layout.need.shared_kv else torch.empty(shape, dtype=dtype, device=device))
+            self.k_scales.append(torch.empty(shape[:4], dtype=torch.uint8, device=device) if self.quantised else None)
+            self.v_scales.append(self.k_scales[-1] if layout.need.shared_kv or not self.quantised
+                                 else torch.empty(shape[:4], dtype=torch.uint8, device=device))
         self.state: List[Optional[torch.Tensor]] = [
             torch.zeros((self.max_seqs, *s.shape), dtype=s.dtype, device=device) if s is not None else None
             for s in states]
@@ -251,16 +272,16 @@ class PagedCache(SlotBook):
                 s.index_copy_(0, slots_long, rows)
 
     def bytes(self) -> int:
-        n = sum(t.numel() * t.element_size() for t in self.k_pools)
-        n += sum(v.numel() * v.element_size() for k, v in zip(self.k_pools, self.v_pools) if v is not k)
+        n = sum(t.numel() * t.element_size() for t in self.k_pools + self.k_scales if t is not None)
+        n += sum(v.numel() * v.element_size() for k, v in zip(self.k_pools + self.k_scales, self.v_pools + self.v_scales) if v is not k)
         return n + sum(s.numel() * s.element_size() for s in self.state if s is not None)
 
     def bytes_per_token(self) -> int:
         """Key and value bytes one token of one sequence occupies over all groups."""
         item = torch.empty((), dtype=self.dtype).element_size()
-        return sum((1 if g.need.shared_kv else 2) * len(g.entries) * g.need.kv_heads * g.need.head_dim * item for g in self.groups)
+        return sum(len(g.entries) * _row_bytes(g.need, item, 1 if self.quantised else 0) for g in self.groups)
 
-    def view(self, entry: int, page_tables: Sequence[torch.Tensor]) -> Optional[KVView]:
+    def view(self, entry: int, page_tables: Sequence[torch.Tensor]) -> Union[KVView, QuantisedKVView, None]:
         """The cache of schedule entry `entry` for the sequences whose page lists (one tensor
         per group, [n_seqs, pages]) are given."""
         w = self.where[entry]
@@ -269,5 +290,32 @@ class PagedCache(SlotBook):
         g, idx = w
         need = self.groups[g].need
         per_entry = self.n_pages * need.kv_heads * self.page_size * need.head_dim
+        if self.quantised:
+            return QuantisedKVView(self.k_pools[g], self.v_pools[g], self.k_scales[g], self.v_scales[g], idx * per_entry, page_tables[g],
+                                   self.page_size, need.kv_heads, need.head_dim)
         return KVView(self.k_pools[g], self.v_pools[g], idx * per_entry, page_tables[g], self.page_size,
                       need.kv_heads, need.head_dim)
+
+    def read(self, entry: int, slot: int) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """What schedule entry `entry` has cached of the sequence in `slot`, as dense rows [tokens, kv_heads, head_dim]: keys, and values
+        (None where they are read out of the key rows).  Rows of pages that a window has given back are zeros.  From an 8-bit
+        cache they come as bfloat16, which holds them exactly."""
+        self._require(slot)
+        where = self.where[entry]
+        if where is None:
+            raise CacheMisuse(f"schedule entry {entry} keeps no keys")
+        need, n = self.groups[where[0]].need, self.length[slot]
+        pages = torch.tensor([self.page_lists[slot][where[0]] or [-1]], dtype=torch.int32, device=self.device)
+        if self.quantised:
+            position = torch.arange(n, dtype=torch.int32, device=self.device)
+            rows = [torch.empty(n, need.kv_heads, need.head_dim, dtype=torch.bfloat16, device=self.device) for _ in range(1 if need.shared_kv else 2)]
+            tables = [pages if g == where[0] else None for g in range(len(self.groups))]
+            with torch.cuda.device(self.device):
+                kernels.dequantise_kv(rows[0], None if need.shared_kv else rows[1], position, torch.zeros_like(position), self.view(entry, tables))
+        else:
+            page = pages[0].long()
+            rows = []
+            for pool in (self.k_pools[where[0]],) + (() if need.shared_kv else (self.v_pools[where[0]],)):
+                x = torch.where((page >= 0).view(-1, 1, 1, 1), pool[where[1], page.clamp(min=0)], torch.zeros((), dtype=pool.dtype, device=pool.device))
+                rows.append(x.transpose(1, 2).reshape(-1, need.kv_heads, need.head_dim)[:n])
+        return rows[0], rows[1] if len(rows) > 1 else None

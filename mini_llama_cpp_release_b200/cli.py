@@ -13,7 +13,7 @@ Option names and meanings follow the reference where it has them (src/main.cpp:2
 not reproducible), `--dump-logits <dir>`, `--device <N>`, `--verbose`.  New: `--random
 <preset|config.json>` runs a model with random weights (written to a temporary folder from
 the configuration and `--weights-seed`) instead of `--model`; `--slots`, `--max-tokens`
-and `--max-batch-tokens` are the engine's sizes.  There is no tokenizer here, so
+and `--max-batch-tokens` are the engine's sizes, `--cache-dtype` what cached keys and values are held in.  There is no tokenizer here, so
 `-p/--prompt <text>` becomes `--tokens "<ids>"` with `;` between sequences; `--backend`,
 `--quant`, `--threads` and `--tokenizer` have nothing to select and are gone.  As in the
 reference, a first argument that is an option means `generate`.
@@ -60,6 +60,8 @@ def add_engine_options(ap: argparse.ArgumentParser) -> None:
                     help="tokens the cache holds (default: what the request needs)")
     ap.add_argument("--slots", type=int, default=None, help="sequences that may be live at once (default: one per 64 cached tokens)")
     ap.add_argument("--max-batch-tokens", type=int, default=None, help="most tokens one step runs at once (default: 16384)")
+    ap.add_argument("--cache-dtype", default=None, choices=["bfloat16", "bf16", "float32", "fp32", "float8_e4m3", "fp8"],
+                    help="element type of cached keys and values (default: --dtype; float8_e4m3 with bfloat16 only)")
 
 
 def resolve_model(args) -> Tuple[str, Optional[str]]:
@@ -85,6 +87,8 @@ def engine_config(args, need_tokens: int):
     if getattr(args, "backend", "cuda") != "cuda":
         raise SystemExit("--backend cpu: this engine runs on a CUDA device only (there is no CPU path)")
     kw = {} if args.max_batch_tokens is None else {"max_batch_tokens": args.max_batch_tokens}
+    if getattr(args, "cache_dtype", None) is not None:
+        kw["cache_dtype"] = args.cache_dtype
     try:
         return EngineConfig(dtype=args.dtype, device=f"cuda:{args.device}", max_tokens=args.max_tokens or need_tokens,
                             max_seqs=args.slots, **kw)

@@ -16,6 +16,7 @@ import torch
 from .. import kernels
 from ..cache.paged import PAGE_SIZE, PagedCache
 from .batch import MiniBatch, SequenceChunk
+from .engine_config import parse_cache_dtype
 from .decode_runner import DecodeRunner, capturing, padded_batch
 from .model import Model
 from .step_info import StepInfo
@@ -28,10 +29,11 @@ class ContextOverflow(ValueError):
 
 class Context:
     def __init__(self, model: Model, max_tokens: int, max_seqs: Optional[int] = None, page_size: int = PAGE_SIZE,
-                 max_batch_tokens: int = 16384):
+                 max_batch_tokens: int = 16384, cache_dtype=None):
         """`max_tokens`: the most tokens live sequences hold at any time, each sequence's
         count rounded up to whole pages of `page_size` tokens.  `max_batch_tokens`: the most
-        tokens one step runs at once; a larger batch is run as several steps."""
+        tokens one step runs at once; a larger batch is run as several steps.  `cache_dtype`: the
+        element type of cached keys and values (`EngineConfig`)."""
         self.model = model
         if max_batch_tokens < 1:
             raise ValueError("max_batch_tokens must be positive")
@@ -39,9 +41,16 @@ class Context:
         rt = model.runtime
         if max_seqs is None:
             max_seqs = min((max_tokens + page_size - 1) // page_size, 4096)
+        cache_dtype = parse_cache_dtype(cache_dtype, rt.dtype)
+        if cache_dtype != rt.dtype:
+            for mixer in model.schedule_mixers():
+                if hasattr(mixer, "cache_need") and mixer.cache_need() is not None and not getattr(mixer, "takes_quantised_cache", False):
+                    raise ValueError(f"an 8-bit cache: the mixer {mixer.name!r} ({type(mixer).__name__}) writes and reads 16-bit keys and values only")
         with torch.cuda.device(rt.device):
             self.cache = PagedCache(model.cache_needs(), model.reads_cache_of(), model.state_specs(), max_tokens,
-                                    max_seqs, rt.dtype, rt.device, page_size)
+                                    max_seqs, cache_dtype, rt.device, page_size)
+            for head_dim in {layout.need.head_dim for layout in self.cache.groups if self.cache.quantised}:
+                kernels.attention_q8_library(head_dim)          # compiled now, not at the first step
         self.max_position = model.config.max_position_embeddings
         self.token_history: Dict[int, List[int]] = {}
         self.n_steps = 0
@@ -93,8 +102,10 @@ class Context:
         widths = [max(1, max(len(cache.page_lists[s][g]) for s in slots)) for g in range(n_groups)]
         # one host buffer (pinned once and reused; an event says when the last copy out of it is done), one copy.
         # Segments: tokens, positions, sequence of each token, first token of each sequence, first position of each
-        # sequence, slots, wanted rows, then one page table per cache group; each 16-byte aligned.
+        # sequence, slots, wanted rows, then one page table per cache group, and for an 8-bit cache the tokens' places among dense
+        # rows; each 16-byte aligned.
         sizes = [n_tokens, n_tokens, n_tokens, B + 1, B, B, len(want_rows)] + [B * w for w in widths]
+        sizes += [n_tokens, n_tokens] if cache.quantised else []         # `StepInfo.token_rows`
         offsets = []
         total = 0
         for size in sizes:
@@ -125,6 +136,10 @@ class Context:
             for b, s in enumerate(slots):
                 pl = cache.page_lists[s][g]
                 table[b, :len(pl)] = pl
+        if cache.quantised:
+            index, row_seq = (host_np[o: o + n_tokens] for o in offsets[-2:])
+            index[:] = np.arange(n_tokens, dtype=np.int32)
+            np.subtract(index, host_np[offsets[1]: offsets[1] + n_tokens], out=row_seq)
         return dict(total=total, offsets=offsets, n_tokens=n_tokens, n_seqs=B, max_q=max_q, max_kv=max_kv,
                     widths=widths, n_want=len(want_rows))
 
@@ -158,12 +173,14 @@ class Context:
             return dev[offsets[i]: offsets[i] + n]
 
         page_tables = [seg(7 + g, B * widths[g]).view(B, widths[g]) for g in range(len(widths))]
+        n_segments = 7 + len(widths)
+        token_rows = (seg(n_segments, n_tokens).view(n_tokens, 1), seg(n_segments + 1, n_tokens)) if len(offsets) > n_segments else None
         slots_dev = seg(5, B)
         return StepInfo(
             n_tokens=n_tokens, n_seqs=B, max_q_len=layout["max_q"], max_kv_len=layout["max_kv"],
             tokens=seg(0, n_tokens), positions=seg(1, n_tokens), tok_seq=seg(2, n_tokens),
             cu_seqlens=seg(3, B + 1), start_pos=seg(4, B), slots=slots_dev, want_rows=seg(6, layout["n_want"]),
-            page_tables=page_tables, slots_long=slots_dev.long() if self.cache.has_state else None,
+            page_tables=page_tables, slots_long=slots_dev.long() if self.cache.has_state else None, token_rows=token_rows,
         )
 
     # A shape of step that comes again (the same numbers of tokens and sequences, the same longest lengths: fixed-size prompts,

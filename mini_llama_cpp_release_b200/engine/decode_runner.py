@@ -83,7 +83,8 @@ class DecodeRunner:
         self.pages_per_seq = max(1, (max_len + self.cache.page_size - 1) // self.cache.page_size)
         n_groups = len(self.cache.groups)
         # one int32 buffer; the per-step inputs come first so that one copy brings them
-        names = [("tokens", B), ("positions", B), ("start_pos", B), ("sample_pos", B),
+        inputs = ["tokens", "positions", "start_pos", "sample_pos"] + (["row_seq"] if self.cache.quantised else [])
+        names = [(name, B) for name in inputs] + [("row_index", B)] * self.cache.quantised + [
                  ("tok_seq", B), ("cu_seqlens", B + 1), ("slots", B), ("want_rows", B), ("seq_ids", B), ("chosen", B),
                  ("counter", 1), ("seed", 2)] + [(f"pages{g}", B * self.pages_per_seq) for g in range(n_groups)]
         self.offsets = {}
@@ -102,12 +103,14 @@ class DecodeRunner:
         h("tok_seq")[:] = torch.arange(B, dtype=torch.int32)
         h("cu_seqlens")[:] = torch.arange(B + 1, dtype=torch.int32)
         h("want_rows")[:] = torch.arange(B, dtype=torch.int32)
+        if self.cache.quantised:
+            h("row_index")[:] = torch.arange(B, dtype=torch.int32)
         for g in range(n_groups):
             h(f"pages{g}")[:] = -1
         self.chosen_dev = self.view("chosen")
         self.chosen_np = self.chosen_host.numpy()
         # the per-step inputs as views made once: slicing a tensor costs microseconds that every step would pay
-        end = self.offsets["sample_pos"][0] + B                     # tokens, positions, start_pos, sample_pos lie first
+        end = self.offsets[inputs[-1]][0] + B                       # the per-step inputs lie first
         self._copy_step_in = kernels.PinnedCopy(self.dev_buf[:end], self.host_buf[:end])
         self._copy_chosen_out = kernels.PinnedCopy(self.chosen_host, self.chosen_dev)
         # the page tables likewise, one per group
@@ -115,7 +118,8 @@ class DecodeRunner:
         self._np_pages = [self.host_np[a].reshape(B, self.pages_per_seq) for a in areas]
         self._copy_pages_in = [kernels.PinnedCopy(self.dev_buf[a], self.host_buf[a]) for a in areas]
         self._np_step = {n: self.host_np[self.offsets[n][0]:self.offsets[n][0] + B]
-                         for n in ("tokens", "positions", "start_pos", "sample_pos")}
+                         for n in inputs}
+        self._rows = np.arange(B, dtype=np.int32)
         self.sync_stream = torch.cuda.current_stream(dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.logits: Optional[torch.Tensor] = None
@@ -141,7 +145,8 @@ class DecodeRunner:
         return StepInfo(n_tokens=B, n_seqs=B, max_q_len=1, max_kv_len=self.max_len,
                         tokens=self.view("tokens"), positions=self.view("positions"), tok_seq=self.view("tok_seq"),
                         cu_seqlens=self.view("cu_seqlens"), start_pos=self.view("start_pos"), slots=self.view("slots"),
-                        want_rows=self.view("want_rows"), page_tables=tables, slots_long=self.slots_long, wants_every_row=True)
+                        want_rows=self.view("want_rows"), page_tables=tables, slots_long=self.slots_long, wants_every_row=True,
+                        token_rows=(self.view("row_index").view(B, 1), self.view("row_seq")) if self.cache.quantised else None)
 
     # ------------------------------------------------------------------ one step's body
     def _body(self) -> None:
@@ -151,6 +156,8 @@ class DecodeRunner:
                                    seed_on_device=self.view("seed"))
         kernels.decode_advance(self.view("chosen"), self.view("tokens"), self.view("positions"), self.view("start_pos"),
                                self.view("sample_pos"), self.history, self.view("counter"))
+        if self.cache.quantised:                      # the next step's `StepInfo.token_rows`
+            torch.sub(self.view("row_index"), self.view("positions"), out=self.view("row_seq"))
 
     def capture(self) -> None:
         """Run the step once eagerly (libraries initialise, tables are built), then capture it.
@@ -193,6 +200,8 @@ class DecodeRunner:
         h("positions")[:] = torch.tensor(lengths, dtype=torch.int32)
         h("start_pos")[:] = h("positions")
         h("sample_pos")[:] = h("positions") + 1
+        if self.cache.quantised:
+            h("row_seq")[:] = h("row_index") - h("positions")
         h("slots")[:] = torch.tensor(list(slots), dtype=torch.int32)
         h("seq_ids")[:] = torch.tensor(list(seq_ids), dtype=torch.int32)
         h("counter")[:] = 0
@@ -243,6 +252,8 @@ class DecodeRunner:
         v["positions"][:] = lengths
         np.copyto(v["start_pos"], v["positions"])
         np.add(v["positions"], 1, out=v["sample_pos"])
+        if self.cache.quantised:
+            np.subtract(self._rows, v["positions"], out=v["row_seq"])
         self._copy_step_in()
         return self._copy_step_in.nbytes
 

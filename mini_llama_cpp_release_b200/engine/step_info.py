@@ -9,7 +9,7 @@ result.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Optional, Tuple
 
 import torch
 
@@ -29,6 +29,11 @@ class StepInfo:
     want_rows: torch.Tensor       # [n_want] packed token rows whose logits are asked for
     page_tables: List[torch.Tensor]   # per cache group: [n_seqs, pages] page of each page index, -1: none
     slots_long: Optional[torch.Tensor] = None   # [n_seqs] int64 copy of `slots`, for indexing state tensors; None when no mixer of the model declared state
+    # With an 8-bit cache, (page lists, sequence numbers) that make row t of dense rows [n_tokens, kv_heads, head_dim] the place of token t's
+    # keys, for the kernels that write a cache of pages: pages of one token, of which token t's is number t.  They look a token up at (its
+    # sequence · pages a list + its position), so lists of one page and t - position for the sequence lead to t.  Part of the
+    # description, which is complete before a step's first kernel: some of those kernels read it ahead of what runs before them.
+    token_rows: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
     wants_every_row: bool = False     # known to the host: `want_rows` is 0, 1, ..., n_tokens - 1
     # what one part leaves for the next part of the same step (a block that has just written the residual stream's
     # 16-bit copy hands it to the block that reads it); keyed by the leaving part's choice, gone with the step

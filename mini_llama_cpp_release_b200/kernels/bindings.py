@@ -1933,7 +1933,7 @@ def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_he
                               keep_first: int = 0, chunk: int = 0):
     """(n_splits, tiles_per_split) of the form with 128 rows a block, or None where it is not for these sizes."""
     group = q_heads // kv_heads
-    if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len * group < 64:
+    if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len < 2 or max_q_len * group < 64:
         return None
     heads = min(group, 128)
     tokens = 128 // heads

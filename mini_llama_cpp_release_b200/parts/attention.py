@@ -117,6 +117,27 @@ class GQAttention(Part):
 
     # ---- the step
     accumulates = True        # forward(..., residual=x) may add the branch into the float32 stream and return None
+    takes_quantised_cache = True
+
+    def write_place(self, step, memory: MixerMemory):
+        """(view, sequence numbers) under which the step's keys and values are written: the cache entry, or for an 8-bit entry dense 16-bit
+        rows that `store` then quantises; (None, ...) when this run writes none."""
+        kv = memory.kv
+        if not memory.writes_cache:
+            return None, step.tok_seq
+        if not isinstance(kv, kernels.QuantisedKVView):
+            return kv, step.tok_seq
+        pages, seq = step.token_rows
+        k = self.runtime.empty(1, step.n_tokens, kv.kv_heads, 1, kv.head_dim)
+        v = k if kv.v_pool is kv.k_pool else self.runtime.empty(1, step.n_tokens, kv.kv_heads, 1, kv.head_dim)
+        return kernels.KVView(k, v, 0, pages, 1, kv.kv_heads, kv.head_dim), seq
+
+    def store(self, place, step, memory: MixerMemory) -> None:
+        """The rows written to `place` into an 8-bit cache entry; any other holds them already."""
+        if place is not None and place is not memory.kv:
+            k = place.k_pool.view(step.n_tokens, place.kv_heads, place.head_dim)
+            v = None if place.v_pool is place.k_pool else place.v_pool.view(step.n_tokens, place.kv_heads, place.head_dim)
+            kernels.quantise_kv(k, v, step.positions, step.tok_seq, memory.kv)
 
     def forward(self, h, step, memory: MixerMemory, residual: Optional[torch.Tensor] = None):
         rt = self.runtime
@@ -126,6 +147,7 @@ class GQAttention(Part):
             self.position.prepare(step.max_kv_len)
         table = getattr(self.position, "table", None)
         q = rt.empty(n, self.H * self.hd)
+        place, tok_seq = self.write_place(step, memory)
         kv_heads = self.KV if memory.writes_cache else 0
         if memory.writes_cache:
             proj, bias = self.qkv, self.bias
@@ -137,22 +159,22 @@ class GQAttention(Part):
         if self.fused and kernels.gemm_rows_takes(n, proj.weight.shape[0], self.hidden) and self.hd % 16 == 0:
             # prompts: tokens as the M operand, a thread of the epilogue holds a token's rotation pairs
             kernels.gemm_tcgen05_rows(h, proj.weight, q, kernels.bindings.EPI_QKV, bias=bias, positions=step.positions,
-                                      tok_seq=step.tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
-                                      kv=memory.kv if memory.writes_cache else None, n_sms=rt.n_sms)
+                                      tok_seq=tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
+                                      kv=place, n_sms=rt.n_sms)
         elif self.fused and (plan := self._few_plan(n, proj.weight.shape[0])) is not None:
             kernels.gemm_few(h, proj.weight, q, kernels.bindings.EPI_QKV, plan, gain, eps, bias=bias, positions=step.positions,
-                             tok_seq=step.tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
-                             kv=memory.kv if memory.writes_cache else None)
+                             tok_seq=tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
+                             kv=place)
         elif self.fused:
             # short epilogues in more blocks beat one long one; the few tiles' K range shared out over clusters of blocks
             splits = kernels.gemm_qkv_cluster_splits(n, proj.weight.shape[0], self.hidden) if n <= 64 else 1
             kernels.gemm_tcgen05(h, proj.weight, q, kernels.bindings.EPI_QKV, splits, bias=bias, positions=step.positions,
-                                 tok_seq=step.tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
-                                 kv=memory.kv if memory.writes_cache else None, n_sms=rt.n_sms,
+                                 tok_seq=tok_seq, rope=table, q_heads=self.H, kv_heads=kv_heads, head_dim=self.hd,
+                                 kv=place, n_sms=rt.n_sms,
                                  block_tokens=16 if n <= 64 else None)
         elif getattr(self.position, "fusable", False):
-            kernels.qkv_post(proj(h, torch.float32), bias, step.positions, step.tok_seq, table, self.H, kv_heads,
-                             self.hd, q, memory.kv if memory.writes_cache else None)
+            kernels.qkv_post(proj(h, torch.float32), bias, step.positions, tok_seq, table, self.H, kv_heads,
+                             self.hd, q, place)
         else:
             # an encoding that is not a table of rotate-half angles: the part rotates the float32 queries and keys
             # itself, after the bias and before the cache write, as the fused forms do
@@ -165,8 +187,8 @@ class GQAttention(Part):
             if nk:
                 qkv[:, nq:nq + nk] = self.position.rotate(qkv[:, nq:nq + nk].reshape(n, kv_heads, self.hd), step.positions,
                                                           out_dtype=torch.float32).reshape(n, nk)
-            kernels.qkv_post(qkv, None, step.positions, step.tok_seq, None, self.H, kv_heads, self.hd, q,
-                             memory.kv if memory.writes_cache else None)
+            kernels.qkv_post(qkv, None, step.positions, tok_seq, None, self.H, kv_heads, self.hd, q, place)
+        self.store(place, step, memory)
         o = rt.empty(n, self.H * self.hd)
         self.attend(q, o, step, memory.kv)
         return self._out(o, residual)
@@ -188,6 +210,10 @@ class GQAttention(Part):
         sinks = getattr(self, "sinks", None)          # float32 [heads] or None: a logit per head that joins every softmax
         chunk = getattr(self, "chunk", None) or 0     # a mask of chunks instead of a window
         softcap = getattr(self, "softcap", None) or 0.0
+        if isinstance(kv, kernels.QuantisedKVView):
+            kernels.attention_quantised(q, o, step.cu_seqlens, step.start_pos, step.n_seqs, step.max_q_len, step.max_kv_len, self.H, kv, self.scale,
+                                        window, sinks=sinks, keep_first=keep, chunk=chunk, softcap=softcap)
+            return
         if self.use_tensor_cores:
             row_tiles, n_splits = kernels.attention_mma_plan(step.max_q_len, step.n_seqs, step.max_kv_len, self.H,
                                                              self.KV, rt.n_sms)
@@ -408,10 +434,12 @@ class SinkAttention(GQAttention):
         k_col = q_col + self.H * self.dim
         v_col = k_col + self.KV * self.dim
         g_col = v_col + self.KV * self.vdim if self.own_kv else k_col
+        place, tok_seq = self.write_place(step, memory)
         kernels.qk_norm_rope_cache(proj, q_col, k_col, v_col, self.q_gain, self.k_gain, self.eps if self.qk_norm else -1.0,
-                                   step.positions, step.tok_seq, table, rot, self.H, kv_heads, self.dim, self.vdim,
-                                   self.value_scale, q, memory.kv if memory.writes_cache else None, q_bias=self.q_bias,
+                                   step.positions, tok_seq, table, rot, self.H, kv_heads, self.dim, self.vdim,
+                                   self.value_scale, q, place, q_bias=self.q_bias,
                                    k_bias=self.k_bias, v_bias=self.v_bias, interleaved=self.interleaved, q_temp=self.q_temp)
+        self.store(place, step, memory)
         o = rt.empty(n, self.H * self.hd)
         self.attend(q, o, step, memory.kv)
         if self.out_gate:
@@ -520,10 +548,12 @@ class DifferentialAttention(SinkAttention):
         k_col = col + self.H * self.dim
         v_col = k_col + self.KV * self.MAPS * self.dim
         g_col = v_col + self.KV * self.vdim if self.own_kv else k_col
-        kernels.qk_norm_rope_cache(proj, col, k_col, v_col, None, None, -1.0, step.positions, step.tok_seq, table, rot, self.H,
-                                   self.KV if self.own_kv else 0, self.dim, self.vdim, 1.0, q, memory.kv if self.own_kv else None,
+        place, tok_seq = self.write_place(step, memory)
+        kernels.qk_norm_rope_cache(proj, col, k_col, v_col, None, None, -1.0, step.positions, tok_seq, table, rot, self.H,
+                                   self.KV if self.own_kv else 0, self.dim, self.vdim, 1.0, q, place,
                                    q_bias=self.q_bias, k_bias=self.k_bias, v_bias=self.v_bias, interleaved=self.interleaved,
                                    maps=self.MAPS)
+        self.store(place, step, memory)
         o = rt.empty(n, self.H * self.hd)
         self.attend(q, o, step, memory.kv)
         act = rt.empty(n, self.heads * self.vdim)
@@ -666,9 +696,10 @@ class LatentAttention(GQAttention):
         qsrc = proj if q_rows is None else q_rows
         table = self.position.table_for(step.max_kv_len) if self.rot and hasattr(self.position, "table_for") else None
         q = rt.empty(n, H * D)
-        kernels.latent_prepare(proj, q_col, col + self.kv_col, self.gain, self.eps, step.positions, step.tok_seq, table, H,
-                               self.dim, self.rot, self.rank, q, memory.kv if memory.writes_cache else None, q_rows=q_rows,
-                               interleaved=self.interleaved)
+        place, tok_seq = self.write_place(step, memory)
+        kernels.latent_prepare(proj, q_col, col + self.kv_col, self.gain, self.eps, step.positions, tok_seq, table, H,
+                               self.dim, self.rot, self.rank, q, place, q_rows=q_rows, interleaved=self.interleaved)
+        self.store(place, step, memory)
         if self.dim:
             # the key expansion on the query's side: q'[t, h, :rank] = W_uk,hᵀ q_plain[t, h]
             kernels.head_project(qsrc, (qsrc.stride(0), self.dim + self.rot), self.w_uk, (self.dim * self.rank, self.rank, 1),
@@ -771,9 +802,11 @@ class ConvKeyAttention(SinkAttention):
         rot = getattr(self.position, "dims", 0) if table is not None else 0
         q = rt.empty(n, self.H * self.hd)
         # the values are the key columns themselves, before norm and rotation
-        kernels.qk_norm_rope_cache(qk, 0, self.n_q, self.n_q, self.q_gain, self.k_gain, self.eps, step.positions, step.tok_seq,
-                                   table, rot, self.H, self.KV, self.dim, self.dim, 1.0, q, memory.kv, whole_row=True,
+        place, tok_seq = self.write_place(step, memory)
+        kernels.qk_norm_rope_cache(qk, 0, self.n_q, self.n_q, self.q_gain, self.k_gain, self.eps, step.positions, tok_seq,
+                                   table, rot, self.H, self.KV, self.dim, self.dim, 1.0, q, place, whole_row=True,
                                    interleaved=self.interleaved)
+        self.store(place, step, memory)
         o = rt.empty(n, self.H * self.hd)
         self.attend(q, o, step, memory.kv)
         return o

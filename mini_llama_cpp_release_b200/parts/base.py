@@ -26,11 +26,11 @@ Interfaces (duck-typed; the classes below document them):
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple
+from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ..kernels import KVView
+from ..kernels import KVView, QuantisedKVView
 
 
 @dataclass(frozen=True)
@@ -80,7 +80,7 @@ class MixerMemory:
     """What the engine hands a mixer at a step: its cache entry (if it declared a cache
     need, or reads another entry's) and its state area [n_slots, *shape] (if it declared
     state).  `writes_cache` is False when the entry belongs to another run of the schedule."""
-    kv: Optional[KVView] = None
+    kv: Union[KVView, QuantisedKVView, None] = None      # (the second with an 8-bit cache, to mixers that say `takes_quantised_cache`)
     state: Optional[torch.Tensor] = None
     writes_cache: bool = True
 

@@ -564,6 +564,10 @@ class ParallelMixer(Part):
     def cache_need(self):
         return next((n for n in (p.cache_need() for p in (self.left, self.right)) if n is not None), None)
 
+    @property
+    def takes_quantised_cache(self) -> bool:
+        return all(getattr(p, "takes_quantised_cache", False) for p in (self.left, self.right) if p.cache_need() is not None)
+
     def state_spec(self):
         return next((s for s in (p.state_spec() for p in (self.left, self.right)) if s is not None), None)
 

@@ -1,0 +1,95 @@
+"""The 8-bit cache without a GPU: options, sizes, views, the format's plain form."""
+import math
+
+import pytest
+import torch
+
+import plain_quantised as plain
+from mini_llama_cpp_release_b200 import EngineConfig, cli
+from mini_llama_cpp_release_b200.cache.paged import PagedCache
+from mini_llama_cpp_release_b200.kernels import KernelError, QuantisedKVView, attention_q8_plan, attention_q8_tcgen05_plan, quantise_kv
+from mini_llama_cpp_release_b200.parts.base import CacheNeed
+
+
+def test_engine_option():
+    for name in ("float8_e4m3", "fp8", torch.float8_e4m3fn):
+        assert EngineConfig(cache_dtype=name).cache_dtype == torch.float8_e4m3fn
+    assert EngineConfig().cache_dtype == torch.bfloat16 and EngineConfig(dtype="fp32").cache_dtype == torch.float32
+    assert EngineConfig(cache_dtype="bf16").cache_dtype == torch.bfloat16
+    for bad in (dict(dtype="fp32", cache_dtype="fp8"), dict(cache_dtype="float32"), dict(dtype="fp32", cache_dtype="bf16"), dict(cache_dtype="e5m2"), dict(cache_dtype=8)):
+        with pytest.raises(ValueError):
+            EngineConfig(**bad)
+
+
+def test_command_line_option():
+    import argparse
+    ap = argparse.ArgumentParser()
+    cli.add_engine_options(ap)
+    assert cli.engine_config(ap.parse_args(["--cache-dtype", "fp8"]), 64).cache_dtype == torch.float8_e4m3fn
+    assert cli.engine_config(ap.parse_args([]), 64).cache_dtype == torch.bfloat16
+    with pytest.raises(SystemExit, match="8-bit cache"):
+        cli.engine_config(ap.parse_args(["--cache-dtype", "fp8", "--dtype", "float32"]), 64)
+
+
+def needs():
+    return [CacheNeed("all", 2, 64), CacheNeed("window", 1, 128, 100, 4), CacheNeed("all", 2, 64), CacheNeed("all", 1, 48, shared_kv=True)]
+
+
+def test_pools_and_views():
+    c = PagedCache(needs(), [None] * 4, [None] * 4, 640, 4, torch.float8_e4m3fn, torch.device("cpu"))
+    assert c.quantised and [tuple(p.shape) for p in c.k_pools] == [(2, 10, 2, 64, 64), (1, 10, 1, 64, 128), (1, 10, 1, 64, 48)]
+    assert [tuple(s.shape) for s in c.v_scales] == [(2, 10, 2, 64), (1, 10, 1, 64), (1, 10, 1, 64)]
+    assert c.v_pools[2] is c.k_pools[2] and c.v_scales[2] is c.k_scales[2] and c.v_scales[0] is not c.k_scales[0]
+    assert c.bytes_per_token() == 2 * 2 * 2 * 65 + 2 * 129 + 49
+    assert c.bytes() == 640 * c.bytes_per_token()
+    tables = [torch.zeros(1, 3, dtype=torch.int32)] * 3
+    v = c.view(2, tables)
+    assert isinstance(v, QuantisedKVView) and v.entry_offset == 10 * 2 * 64 * 64 and v.k_scale is c.k_scales[0] and v.pages_per_seq == 3
+    wide = PagedCache(needs(), [None] * 4, [None] * 4, 640, 4, torch.bfloat16, torch.device("cpu"))
+    assert not wide.quantised and wide.k_scales == [None] * 3 and wide.bytes_per_token() == 2 * (2 * 2 * 2 * 64 + 2 * 128 + 48)
+    assert wide.bytes() == 640 * wide.bytes_per_token()
+
+
+@pytest.mark.parametrize("head_dim,page", [(40, 64), (272, 64), (64, 32)])
+def test_sizes_it_does_not_take(head_dim, page):
+    with pytest.raises(ValueError, match="8-bit cache"):
+        PagedCache([CacheNeed("all", 1, head_dim)], [None], [None], 640, 4, torch.float8_e4m3fn, torch.device("cpu"), page)
+
+
+def test_a_cache_on_the_host_is_refused():
+    c = PagedCache(needs()[:1], [None], [None], 640, 4, torch.float8_e4m3fn, torch.device("cpu"))
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(KernelError, match="CUDA"):
+        quantise_kv(torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), i, i, c.view(0, [torch.zeros(1, 1, dtype=torch.int32)]))
+
+
+def test_plans_cover_every_key():
+    for q_len in (1, 2, 5, 40, 700):
+        for seqs in (1, 3, 64, 300):
+            for keys in (1, 64, 65, 2000, 131072):
+                for heads, kv_heads, hd in ((14, 2, 64), (28, 4, 128), (8, 8, 16), (40, 1, 256), (64, 1, 64)):
+                    for mask in (dict(), dict(window=100), dict(window=5000, keep_first=70), dict(chunk=256)):
+                        rows, n, per, cluster = attention_q8_plan(q_len, seqs, max(keys, q_len), heads, kv_heads, hd, 148, **mask)
+                        tiles = (max(keys, q_len) + 63) // 64
+                        assert rows in (8, 16, 64) and n >= 1 and per >= 1
+                        assert n * per >= tiles or mask, (q_len, seqs, keys)
+                        assert not cluster or (1 < n <= 8 and rows != 64)
+                        p = attention_q8_tcgen05_plan(q_len, seqs, max(keys, q_len), heads, kv_heads, hd, 148, **mask)
+                        assert p is None or p[0] >= 1 and (p[0] * p[1] >= tiles or mask)
+
+
+def test_the_plain_form_of_the_format():
+    values = plain.code_values()
+    assert values[0x7e] == 448 and values[1] == 2.0 ** -9 and values[8] == 2.0 ** -6 and math.isnan(values[0x7f]) and values[0xff].isnan()
+    x = torch.tensor([[448.0, 1.0], [449.0, -449.0], [0.0, 0.0], [math.inf, 1.0], [1e-45, 0.0], [3.4e38, -3.4e38]])
+    codes, scale = plain.quantise(x)
+    assert scale.tolist() == [127, 128, 27, 255, 27, 246]
+    back = plain.values(codes, scale)
+    assert back[0].tolist() == [448, 1] and back[1].tolist() == [448, -448] and back[2].tolist() == [0, 0] and back[3].isnan().all()
+    # 3.4e38 is 511.6 times 2^119: it saturates at 448
+    assert back[5].tolist() == [448 * 2.0 ** 119, -448 * 2.0 ** 119]
+    # a rounding is off by at most half a step: 2^-4 of the number, or half of the smallest step of its row
+    x = torch.randn(400, 64, dtype=torch.float64) * torch.exp2(torch.randint(-30, 30, (400, 1)).double())
+    codes, scale = plain.quantise(x)
+    step = torch.exp2(scale.double() - 127)[:, None] * 2.0 ** -9
+    assert ((plain.values(codes, scale) - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, step / 2)).all()
