@@ -4,7 +4,7 @@ from __future__ import annotations
 import ctypes
 import functools
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional, Tuple
 
 import torch
@@ -1781,7 +1781,7 @@ def gemm_tcgen05(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, epilogue: 
 
 # ------------------------------------------------------------------ the 8-bit cache
 
-@dataclass
+@dataclass(frozen=True)
 class QuantisedKVView:
     """Where one cache entry's keys and values are in an 8-bit cache: pools of e4m3 numbers
     [entries][pages][kv_heads][page_size][head_dim] and of their rows' scale bytes [entries][pages][kv_heads][page_size] (byte b
@@ -1796,60 +1796,67 @@ class QuantisedKVView:
     page_size: int
     kv_heads: int
     head_dim: int
+    device: int = field(init=False, default=-1, repr=False, compare=False)       # the CUDA device's number, once `check` has passed
 
     @property
     def pages_per_seq(self) -> int:
         return self.page_table.shape[1]
 
+    def check(self) -> int:
+        """Once a view: types, devices, and that pools, scales and offset belong together.  Returns the device's number."""
+        if self.device >= 0:
+            return self.device
+        k, v, ks, vs, table = self.k_pool, self.v_pool, self.k_scale, self.v_scale, self.page_table
+        device = k.get_device()
+        if device < 0:
+            raise KernelError("this engine runs on a CUDA device only: got a cache on " + str(k.device))
+        if v.get_device() != device or ks.get_device() != device or vs.get_device() != device or table.get_device() != device:
+            raise KernelError(f"the parts of an 8-bit cache lie on different devices: {k.device}, {v.device}, {ks.device}, {vs.device}, {table.device}")
+        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
+            raise KernelError(f"an 8-bit cache holds float8_e4m3fn beside scales in uint8, not {k.dtype}, {v.dtype} and {ks.dtype}, {vs.dtype}")
+        shape = k.shape
+        if len(shape) != 5 or shape[2:] != (self.kv_heads, self.page_size, self.head_dim) or v.shape != shape or ks.shape != shape[:4] or vs.shape != shape[:4]:
+            raise KernelError(f"pools {tuple(shape)}, {tuple(v.shape)} and scales {tuple(ks.shape)}, {tuple(vs.shape)} do not "
+                              f"fit {self.kv_heads} kv heads, pages of {self.page_size} and heads of {self.head_dim}")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise KernelError("the pools of an 8-bit cache are dense")
+        per_entry = shape[1] * self.kv_heads * self.page_size * self.head_dim
+        if self.entry_offset < 0 or (per_entry and (self.entry_offset % per_entry or self.entry_offset // per_entry >= shape[0])):
+            raise KernelError(f"an entry starts at a multiple of {per_entry} numbers below {shape[0]} of them, not at {self.entry_offset}")
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+            raise KernelError("page lists are a dense int32 tensor [n_seqs, pages]")
+        object.__setattr__(self, "device", device)
+        return device
 
-def _check_quantised(kv: QuantisedKVView, *others: Optional[torch.Tensor]) -> None:
-    """What a kernel cannot see for itself: types, devices, and that pools, scales and offset belong together."""
-    device = kv.k_pool.device
-    if device.type != "cuda":
-        raise KernelError("this engine runs on a CUDA device only: got a cache on " + str(device))
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"the cache lies on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in (kv.v_pool, kv.k_scale, kv.v_scale, kv.page_table) + others:
-        if t is not None and t.device != device:
-            raise KernelError(f"tensors on different devices: {t.device} and {device}")
-    if kv.k_pool.dtype != torch.float8_e4m3fn or kv.v_pool.dtype != torch.float8_e4m3fn:
-        raise KernelError(f"an 8-bit cache holds float8_e4m3fn, not {kv.k_pool.dtype} and {kv.v_pool.dtype}")
-    if kv.k_scale.dtype != torch.uint8 or kv.v_scale.dtype != torch.uint8:
-        raise KernelError("the scales of an 8-bit cache are bytes (uint8)")
-    shape = kv.k_pool.shape
-    if len(shape) != 5 or tuple(shape[2:]) != (kv.kv_heads, kv.page_size, kv.head_dim) or kv.v_pool.shape != shape \
-            or kv.k_scale.shape != shape[:4] or kv.v_scale.shape != shape[:4]:
-        raise KernelError(f"pools {tuple(shape)}, {tuple(kv.v_pool.shape)} and scales {tuple(kv.k_scale.shape)}, {tuple(kv.v_scale.shape)} do not "
-                          f"fit {kv.kv_heads} kv heads, pages of {kv.page_size} and heads of {kv.head_dim}")
-    per_entry = shape[1] * kv.kv_heads * kv.page_size * kv.head_dim
-    if not (kv.k_pool.is_contiguous() and kv.v_pool.is_contiguous() and kv.k_scale.is_contiguous() and kv.v_scale.is_contiguous()):
-        raise KernelError("the pools of an 8-bit cache are dense")
-    if kv.entry_offset < 0 or (per_entry and (kv.entry_offset % per_entry or kv.entry_offset // per_entry >= shape[0])):
-        raise KernelError(f"an entry starts at a multiple of {per_entry} numbers below {shape[0]} of them, not at {kv.entry_offset}")
-    if kv.page_table.dtype != torch.int32 or kv.page_table.dim() != 2 or not kv.page_table.is_contiguous():
-        raise KernelError("page lists are a dense int32 tensor [n_seqs, pages]")
+
+def _on_device(device: int, *tensors: Optional[torch.Tensor]) -> None:
+    """All of them on the cache's device, and that the current one: the kernels run on its current stream."""
+    if device != torch.cuda.current_device():
+        raise KernelError(f"the cache lies on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"a tensor on {t.device} with a cache on cuda:{device}")
 
 
 def _quantised_rows(what: str, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor,
                     kv: QuantisedKVView) -> tuple:
-    _check_quantised(kv, k, v, positions, tok_seq)
-    n = k.shape[0]
-    for t in (k, v):
-        if t is not None and (tuple(t.shape) != (n, kv.kv_heads, kv.head_dim) or t.dtype != k.dtype or (t.numel() and t.stride(2) != 1)):
-            raise KernelError(f"{what}: rows [tokens, {kv.kv_heads}, {kv.head_dim}] of one type with the head's numbers side by side, got "
-                              f"{tuple(t.shape)} {t.dtype} with strides {t.stride()}")
-    if v is None and kv.v_pool.data_ptr() != kv.k_pool.data_ptr():
-        raise KernelError(f"{what}: the entry has values of its own")
-    if v is not None and kv.v_pool.data_ptr() == kv.k_pool.data_ptr():
-        raise KernelError(f"{what}: the entry's values are its key rows; there are no others")
-    for t in (positions, tok_seq):
-        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
-            raise KernelError(f"{what}: positions and sequences are dense int32, one per token")
-    vs = v if v is not None else k
-    return (k.data_ptr(), _ptr(v), dtype_code(k.dtype), k.stride(0), k.stride(1), vs.stride(0), vs.stride(1), positions.data_ptr(),
-            tok_seq.data_ptr(), n, kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
-            kv.page_table.data_ptr(), kv.page_table.shape[0], kv.page_table.shape[1], kv.entry_offset, kv.k_pool.shape[1], kv.page_size,
-            kv.kv_heads, kv.head_dim, _stream())
+    _on_device(kv.check(), k, v, positions, tok_seq)
+    n = positions.numel()
+    shape = (n, kv.kv_heads, kv.head_dim)
+    ks = k.stride()
+    vs = ks if v is None else v.stride()
+    if k.shape != shape or (n and ks[2] != 1) or (v is not None and (v.shape != shape or v.dtype != k.dtype or (n and vs[2] != 1))):
+        raise KernelError(f"{what}: rows [tokens, {kv.kv_heads}, {kv.head_dim}] of one type with the head's numbers side by side, got {tuple(k.shape)} {k.dtype}, "
+                          f"strides {ks}" + ("" if v is None else f", and {tuple(v.shape)} {v.dtype}, strides {vs}"))
+    shared = kv.v_pool.data_ptr() == kv.k_pool.data_ptr()
+    if shared != (v is None):
+        raise KernelError(f"{what}: the entry's values are its key rows; there are no others" if shared else f"{what}: the entry has values of its own")
+    if positions.dtype != torch.int32 or tok_seq.dtype != torch.int32 or tok_seq.numel() != n or not positions.is_contiguous() or not tok_seq.is_contiguous():
+        raise KernelError(f"{what}: positions and sequences are dense int32, one per token")
+    table = kv.page_table.shape
+    return (k.data_ptr(), _ptr(v), dtype_code(k.dtype), ks[0], ks[1], vs[0], vs[1], positions.data_ptr(), tok_seq.data_ptr(), n, kv.k_pool.data_ptr(),
+            kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), table[0], table[1], kv.entry_offset,
+            kv.k_pool.shape[1], kv.page_size, kv.kv_heads, kv.head_dim, _stream())
 
 
 def quantise_kv(k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor, kv: QuantisedKVView) -> None:
@@ -1890,6 +1897,7 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     return lib
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                       keep_first: int = 0, chunk: int = 0):
     """(rows, n_splits, tiles_per_split, in_cluster) of the form without scratch pages: 8, 16 or 64 rows a block, tiles of 64 keys shared out
@@ -1929,6 +1937,7 @@ def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
         return None
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
     """(n_splits, tiles_per_split) of the form with 128 rows a block, or None where it is not for these sizes."""
@@ -1957,18 +1966,19 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     `max_q_len`, `max_kv_len`: bounds of a sequence's new tokens and of its keys with them.  `window`, `sinks`, `keep_first`, `chunk` and
     `softcap` as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows behind the
     last sequence's are left as they are."""
-    _check_quantised(kv, q, out, cu_seqlens, start_pos, sinks)
-    require_cuda(q, out, cu_seqlens, start_pos, sinks)
+    device = kv.check()
+    _on_device(device, q, out, cu_seqlens, start_pos, sinks)
     n = q.shape[0]
+    if not (q.is_contiguous() and out.is_contiguous() and cu_seqlens.is_contiguous() and start_pos.is_contiguous()):
+        raise KernelError("attention over an 8-bit cache takes dense tensors")
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise KernelError("attention over an 8-bit cache takes bfloat16 queries and output")
     if q_heads <= 0 or q_heads % kv.kv_heads or q.numel() != n * q_heads * kv.head_dim or out.shape != q.shape:
         raise KernelError(f"attention over an 8-bit cache: {q_heads} query heads on {kv.kv_heads} kv heads of {kv.head_dim}, q {tuple(q.shape)}, out {tuple(out.shape)}")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != q_heads):
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != q_heads or not sinks.is_contiguous()):
         raise KernelError("attention over an 8-bit cache: sinks are one float32 per query head")
-    for t, size in ((cu_seqlens, n_seqs + 1), (start_pos, n_seqs)):
-        if t.dtype != torch.int32 or t.numel() < size:
-            raise KernelError(f"attention over an 8-bit cache: sequence bounds are int32, {size} of them")
+    if cu_seqlens.dtype != torch.int32 or start_pos.dtype != torch.int32 or cu_seqlens.numel() <= n_seqs or start_pos.numel() < n_seqs:
+        raise KernelError(f"attention over an 8-bit cache: sequence bounds are int32, {n_seqs + 1} first tokens and {n_seqs} first positions")
     if kv.page_size != 64 or kv.page_table.shape[0] < n_seqs:
         raise KernelError(f"attention over an 8-bit cache: pages of 64 tokens and a page list per sequence, got pages of {kv.page_size} and "
                           f"{kv.page_table.shape[0]} lists for {n_seqs}")
