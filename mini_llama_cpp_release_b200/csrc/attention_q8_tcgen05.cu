@@ -473,13 +473,13 @@ extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_
 extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_seqlens, const int* start_pos, int n_seqs, int n_tokens, int max_q_len,
                                         int q_heads, int kv_heads, int hd, float scale, int window, int keep_first, int chunk, float softcap,
                                         const float* sinks, int n_splits, int tiles_per_split, float* part_ml, float* part_o, void* dense, int dense_tiles,
-                                        void* k_pool, void* v_pool, void* k_scale, void* v_scale, const int* page_table, int pages_per_seq,
+                                        void* k_pool, void* v_pool, void* k_scale, void* v_scale, const int* page_table, int n_lists, int pages_per_seq,
                                         long long entry_offset, long long n_pages, int page_size, int* status, void* stream) {
 #if MLC_Q8_TCGEN05
     if (hd != X_HD || page_size != X_KEYS) return MLC_ERR_UNSUPPORTED;
     if (chunk < 0 || (chunk > 0 && window > 0) || !(softcap >= 0.0f)) return MLC_ERR_UNSUPPORTED;
     if (n_seqs <= 0 || n_tokens <= 0 || max_q_len <= 0) return 0;
-    if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || status == nullptr || n_pages <= 0 || n_pages > 0x7fffffffll || pages_per_seq < 0) return MLC_ERR_BAD_SIZE;
+    if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || status == nullptr || n_pages <= 0 || n_pages > 0x7fffffffll || pages_per_seq < 0 || n_lists < n_seqs) return MLC_ERR_BAD_SIZE;
     if (!(scale > 0.0f) || window < 0 || n_splits < 1 || tiles_per_split < 1) return MLC_ERR_BAD_SIZE;
     if (n_splits > 1 && (part_ml == nullptr || part_o == nullptr)) return MLC_ERR_BAD_SIZE;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)dense) & 15) return MLC_ERR_BAD_SIZE;

@@ -83,6 +83,9 @@ def require_cuda(*tensors: Optional[torch.Tensor]) -> None:
             raise KernelError("kernels take dense row-major tensors; got strides " + str(t.stride()))
 
 
+# a `QuantisedKVView`'s pools, scales, page lists [sequences][pages a list], offset, pages of an entry, tokens of a page
+QUANTISED_ARGS = (c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int)
+
 _core = None
 
 
@@ -147,8 +150,8 @@ def core() -> ctypes.CDLL:
             "mlc_argmax_split": [P, I, I, P, P, P, P, P],
             "mlc_sample": [P, I, I, F, I, c_ulonglong, P, P, P, P, P],
             "mlc_decode_advance": [P, I, P, P, P, P, P, P, I, P],
-            "mlc_quantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, P, P, P, P, P, I, I, LL, LL, I, I, I, P],
-            "mlc_dequantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, P, P, P, P, P, I, I, LL, LL, I, I, I, P],
+            "mlc_quantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, *QUANTISED_ARGS, I, I, P],
+            "mlc_dequantise_kv": [P, P, I, LL, LL, LL, LL, P, P, I, *QUANTISED_ARGS, I, I, P],
         }
         for name, args in sigs.items():
             fn = getattr(lib, name)
@@ -1796,7 +1799,8 @@ class QuantisedKVView:
     page_size: int
     kv_heads: int
     head_dim: int
-    device: int = field(init=False, default=-1, repr=False, compare=False)       # the CUDA device's number, once `check` has passed
+    device: int = field(init=False, default=-1, repr=False, compare=False)       # the CUDA device's number, once `check` has passed, and
+    args: tuple = field(init=False, default=(), repr=False, compare=False)       # what every entry point takes of the view, in their order
 
     @property
     def pages_per_seq(self) -> int:
@@ -1815,7 +1819,8 @@ class QuantisedKVView:
         if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or ks.dtype != torch.uint8 or vs.dtype != torch.uint8:
             raise KernelError(f"an 8-bit cache holds float8_e4m3fn beside scales in uint8, not {k.dtype}, {v.dtype} and {ks.dtype}, {vs.dtype}")
         shape = k.shape
-        if len(shape) != 5 or shape[2:] != (self.kv_heads, self.page_size, self.head_dim) or v.shape != shape or ks.shape != shape[:4] or vs.shape != shape[:4]:
+        if len(shape) != 5 or v.shape != shape or shape[2] != self.kv_heads or shape[3] != self.page_size or shape[4] != self.head_dim \
+                or ks.shape != shape[:4] or vs.shape != shape[:4]:
             raise KernelError(f"pools {tuple(shape)}, {tuple(v.shape)} and scales {tuple(ks.shape)}, {tuple(vs.shape)} do not "
                               f"fit {self.kv_heads} kv heads, pages of {self.page_size} and heads of {self.head_dim}")
         if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
@@ -1825,6 +1830,8 @@ class QuantisedKVView:
             raise KernelError(f"an entry starts at a multiple of {per_entry} numbers below {shape[0]} of them, not at {self.entry_offset}")
         if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
             raise KernelError("page lists are a dense int32 tensor [n_seqs, pages]")
+        object.__setattr__(self, "args", (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
+                                          self.entry_offset, shape[1], self.page_size))
         object.__setattr__(self, "device", device)
         return device
 
@@ -1848,15 +1855,14 @@ def _quantised_rows(what: str, k: torch.Tensor, v: Optional[torch.Tensor], posit
     if k.shape != shape or (n and ks[2] != 1) or (v is not None and (v.shape != shape or v.dtype != k.dtype or (n and vs[2] != 1))):
         raise KernelError(f"{what}: rows [tokens, {kv.kv_heads}, {kv.head_dim}] of one type with the head's numbers side by side, got {tuple(k.shape)} {k.dtype}, "
                           f"strides {ks}" + ("" if v is None else f", and {tuple(v.shape)} {v.dtype}, strides {vs}"))
-    shared = kv.v_pool.data_ptr() == kv.k_pool.data_ptr()
+    args = kv.args
+    shared = args[0] == args[1]
     if shared != (v is None):
         raise KernelError(f"{what}: the entry's values are its key rows; there are no others" if shared else f"{what}: the entry has values of its own")
     if positions.dtype != torch.int32 or tok_seq.dtype != torch.int32 or tok_seq.numel() != n or not positions.is_contiguous() or not tok_seq.is_contiguous():
         raise KernelError(f"{what}: positions and sequences are dense int32, one per token")
-    table = kv.page_table.shape
-    return (k.data_ptr(), _ptr(v), dtype_code(k.dtype), ks[0], ks[1], vs[0], vs[1], positions.data_ptr(), tok_seq.data_ptr(), n, kv.k_pool.data_ptr(),
-            kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), table[0], table[1], kv.entry_offset,
-            kv.k_pool.shape[1], kv.page_size, kv.kv_heads, kv.head_dim, _stream())
+    return (k.data_ptr(), _ptr(v), dtype_code(k.dtype), ks[0], ks[1], vs[0], vs[1], positions.data_ptr(), tok_seq.data_ptr(), n, *args, kv.kv_heads, kv.head_dim,
+            _stream())
 
 
 def quantise_kv(k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, tok_seq: torch.Tensor, kv: QuantisedKVView) -> None:
@@ -1886,9 +1892,9 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     if lib is None:
         lib = _build.attention_q8_library(head_dim)
         P, I, F, LL = c_void_p, c_int, c_float, c_longlong
-        lib.mlc_attention_q8.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, I, P, P, P, P, P, P, P, I, LL, LL, I, P, P]
+        lib.mlc_attention_q8.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, I, P, P, *QUANTISED_ARGS, P, P]
         lib.mlc_attention_q8.restype = c_int
-        lib.mlc_attention_q8_tcgen05.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, P, P, P, I, P, P, P, P, P, I, LL, LL, I, P, P]
+        lib.mlc_attention_q8_tcgen05.argtypes = [P, P, P, P, I, I, I, I, I, I, F, I, I, I, F, P, I, I, P, P, P, I, *QUANTISED_ARGS, P, P]
         lib.mlc_attention_q8_tcgen05.restype = c_int
         lib.mlc_attention_q8_head_dim.restype = c_int
         if lib.mlc_attention_q8_head_dim() != head_dim:
@@ -1897,7 +1903,6 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     return lib
 
 
-@functools.lru_cache(maxsize=4096)
 def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                       keep_first: int = 0, chunk: int = 0):
     """(rows, n_splits, tiles_per_split, in_cluster) of the form without scratch pages: 8, 16 or 64 rows a block, tiles of 64 keys shared out
@@ -1937,7 +1942,6 @@ def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
         return None
 
 
-@functools.lru_cache(maxsize=4096)
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
     """(n_splits, tiles_per_split) of the form with 128 rows a block, or None where it is not for these sizes."""
@@ -1956,6 +1960,12 @@ def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_he
     wanted = max(1, n_sms // blocks)
     per_split = max(8, (longest + wanted - 1) // wanted)
     return (longest + per_split - 1) // per_split, per_split
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_q8_form(*sizes) -> tuple:
+    """What a call of these sizes runs: `attention_q8_tcgen05_plan`, or where that is None `attention_q8_plan`."""
+    return attention_q8_tcgen05_plan(*sizes) or attention_q8_plan(*sizes)
 
 
 def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Tensor, start_pos: torch.Tensor, n_seqs: int, max_q_len: int,
@@ -1986,33 +1996,36 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
         raise KernelError(f"attention over an 8-bit cache: scale {scale}, window {window}, keep_first {keep_first}, chunk {chunk}, softcap {softcap}")
     if n == 0 or n_seqs <= 0 or max_q_len <= 0:
         return
-    lib = attention_q8_library(kv.head_dim)
-    sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, kv.head_dim, _sm_count(q.device), window, keep_first, chunk)
-    prompt = attention_q8_tcgen05_plan(*sizes)
-    dense, in_cluster = None, False
-    if prompt is not None:
+    lib = _attn_q8_libs.get(kv.head_dim) or attention_q8_library(kv.head_dim)
+    sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, kv.head_dim, _sm_counts.get(device) or _sm_count(q.device), window, keep_first, chunk)
+    form = _attention_q8_form(*sizes)
+    args = kv.args
+    dense = None
+    if len(form) == 2:
         # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
-        dense_tiles = max(1, kv.pages_per_seq)
+        dense_tiles = max(1, args[6])
         dense = _spare_rows(n_seqs * kv.kv_heads * dense_tiles * 128 * kv.head_dim, q.device)
+        if dense is None:
+            form = attention_q8_plan(*sizes)
     if dense is not None:
-        n_splits, per_split = prompt
+        (n_splits, per_split), in_cluster = form, False
     else:
-        rows, n_splits, per_split, in_cluster = attention_q8_plan(*sizes)
+        rows, n_splits, per_split, in_cluster = form
     part_ml = part_o = None
     joined_later = n_splits > 1 and not in_cluster
     if joined_later:
         part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
         part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
-    head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, float(scale),
-            int(window), int(keep_first), int(chunk), float(softcap), _ptr(sinks))
-    parts = (n_splits, per_split, _ptr(part_ml), _ptr(part_o))
-    tail = (kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), kv.page_table.data_ptr(), kv.pages_per_seq, kv.entry_offset,
-            kv.k_pool.shape[1], kv.page_size, gemm_status(q.device).data_ptr(), _stream())
+    status = _status.get(device)
+    if status is None:
+        status = gemm_status(q.device)
+    head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, scale, window,
+            keep_first, chunk, softcap, _ptr(sinks))
     if dense is not None:
-        rc = lib.mlc_attention_q8_tcgen05(*head, *parts, dense.data_ptr(), dense_tiles, *tail)
+        rc = lib.mlc_attention_q8_tcgen05(*head, n_splits, per_split, _ptr(part_ml), _ptr(part_o), dense.data_ptr(), dense_tiles, *args, status.data_ptr(), _stream())
         count_launches(1)
     else:
-        rc = lib.mlc_attention_q8(*head, rows, *parts, *tail)
+        rc = lib.mlc_attention_q8(*head, rows, n_splits, per_split, _ptr(part_ml), _ptr(part_o), *args, status.data_ptr(), _stream())
     _check(rc, "attention over an 8-bit cache")
     if joined_later:
         count_launches(1)

@@ -93,3 +93,26 @@ def test_the_plain_form_of_the_format():
     codes, scale = plain.quantise(x)
     step = torch.exp2(scale.double() - 127)[:, None] * 2.0 ** -9
     assert ((plain.values(codes, scale) - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, step / 2)).all()
+
+
+def test_argument_lists_are_the_kernels():
+    """The declared argument types of each entry point against its C signature, one by one."""
+    import os
+    import re
+    from ctypes import c_float, c_int, c_longlong, c_void_p
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    root = os.path.dirname(bindings._build.__file__)
+    names = {"P": c_void_p, "I": c_int, "F": c_float, "LL": c_longlong}
+    with open(bindings.__file__) as f:
+        text = f.read()
+    for entry, source in (("mlc_attention_q8", "attention_q8.cu"), ("mlc_attention_q8_tcgen05", "attention_q8_tcgen05.cu"),
+                          ("mlc_quantise_kv", "kv_quantise.cu"), ("mlc_dequantise_kv", "kv_quantise.cu")):
+        with open(os.path.join(root, source)) as f:
+            signature = re.search(r'extern "C" int ' + entry + r"\(([^)]*)\) \{", f.read()).group(1)
+        want = [c_void_p if "*" in a else c_longlong if a.startswith("long long") else c_float if a.startswith("float") else c_int
+                for a in (x.strip() for x in signature.replace("\n", " ").split(","))]
+        declared = (re.search(rf'"{entry}": \[([^\]]*)\]', text) or re.search(rf"lib\.{entry}\.argtypes = \[([^\]]*)\]", text)).group(1)
+        got = []
+        for a in (x.strip() for x in declared.split(",")):
+            got += bindings.QUANTISED_ARGS if a == "*QUANTISED_ARGS" else [names[a]]
+        assert got == want, entry
