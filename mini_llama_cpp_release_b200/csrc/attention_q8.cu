@@ -20,8 +20,9 @@
 //         O^T: lane (g, t) holds of its four keys the numbers g·hd/8 ..., two keys' bytes interleaved before the conversion.
 //   more rows (attention_q8_kernel): 64 rows a block, 16 a warp, S = Q K^T and O = P V with the same orders of numbers; every warp reads every tile.
 // A block has four such warps and one that asks for tiles (64 keys, a page) by bulk copies into a ring: a page's keys of one head are
-// contiguous, 64·hd bytes, and its scales 64.  The tiles of a sequence are shared out over blocks in runs of `tiles_per_split`, whatever
-// the longest sequence is, so that ragged batches come out even; q8_combine_kernel joins them.
+// contiguous, 64·hd bytes, and its scales 64.  The tiles of a sequence are shared out over blocks: where all blocks run at once in equal shares, else
+// in runs of `tiles_per_split`, whatever the longest sequence is, so that ragged batches come out even.  The splits join inside a cluster, or in
+// q8_combine_kernel.
 //
 // Keys of a missing page, and keys behind a row, are not seen; a row that sees no key gives zeros.  Bytes of a page that lie behind the
 // sequence's last key may be anything (NaN among it): their scores are replaced and their values' codes zeroed.
@@ -160,9 +161,13 @@ __device__ __forceinline__ Q8Block q8_block(const Q8Args& a) {
     k.walk.tile_begin = q8_lowest(a, k.p_first) / Q_TILE;
     k.walk.head_tiles = min(k.walk.tile_begin, (k.keep + Q_TILE - 1) / Q_TILE);
     k.walk.n_tiles = k.walk.head_tiles + k.p_last / Q_TILE + 1 - k.walk.tile_begin;
-    // (the last split goes to the end, however long the sequence turns out to be)
-    k.j_begin = k.split * a.tiles_per_split;
-    k.j_end = k.split == a.n_splits - 1 ? k.walk.n_tiles : min(k.walk.n_tiles, k.j_begin + a.tiles_per_split);
+    if (a.tiles_per_split > 0) {           // (the last split goes to the end, however long the sequence turns out to be)
+        k.j_begin = k.split * a.tiles_per_split;
+        k.j_end = k.split == a.n_splits - 1 ? k.walk.n_tiles : min(k.walk.n_tiles, k.j_begin + a.tiles_per_split);
+    } else {
+        k.j_begin = (int)((long long)k.walk.n_tiles * k.split / a.n_splits);
+        k.j_end = (int)((long long)k.walk.n_tiles * (k.split + 1) / a.n_splits);
+    }
     return k;
 }
 
@@ -869,7 +874,7 @@ extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_
 
 // q, out: bfloat16 [n_tokens][q_heads · head_dim], 16-byte aligned.  The entry starts `entry_offset` codes into the pools, which hold
 // `n_pages` pages of 64 tokens an entry.  rows: 8, 16 or 64 a block.  tiles_per_split: tiles of 64 keys a block
-// walks (the last of the n_splits goes on to the end); more than one need part_ml (n_tokens · q_heads · n_splits · 2 floats) and part_o
+// walks (the last of the n_splits goes on to the end), or 0: equal shares of each sequence's own; more than one need part_ml (n_tokens · q_heads · n_splits · 2 floats) and part_o
 // (n_tokens · q_heads · n_splits · head_dim); without part_ml up to 8 splits (of 8 or 16 rows a block) join inside a cluster.  sinks: null or a float per query head.
 extern "C" int mlc_attention_q8(const void* q, void* out, const int* cu_seqlens, const int* start_pos, int n_seqs, int n_tokens, int max_q_len,
                                 int q_heads, int kv_heads, int hd, float scale, int window, int keep_first, int chunk, float softcap,
@@ -880,7 +885,7 @@ extern "C" int mlc_attention_q8(const void* q, void* out, const int* cu_seqlens,
     if (chunk < 0 || (chunk > 0 && window > 0) || !(softcap >= 0.0f)) return MLC_ERR_UNSUPPORTED;
     if (n_seqs <= 0 || n_tokens <= 0 || max_q_len <= 0) return 0;
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || status == nullptr || n_pages <= 0 || n_pages > 0x7fffffffll || pages_per_seq < 0 || n_lists < n_seqs) return MLC_ERR_BAD_SIZE;
-    if (!(scale > 0.0f) || window < 0 || n_splits < 1 || tiles_per_split < 1 || n_seqs > 65535) return MLC_ERR_BAD_SIZE;
+    if (!(scale > 0.0f) || window < 0 || n_splits < 1 || tiles_per_split < 0 || n_seqs > 65535) return MLC_ERR_BAD_SIZE;
     const bool in_cluster = n_splits > 1 && part_ml == nullptr;
     if (in_cluster ? n_splits > Q_CLUSTER || rows == 64 : n_splits > 1 && part_o == nullptr) return MLC_ERR_BAD_SIZE;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15) return MLC_ERR_BAD_SIZE;

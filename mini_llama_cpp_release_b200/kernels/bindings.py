@@ -1905,10 +1905,17 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
 
 def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                       keep_first: int = 0, chunk: int = 0):
-    """(rows, n_splits, tiles_per_split, in_cluster) of the form without scratch pages: 8, 16 or 64 rows a block, tiles of 64 keys shared out
-    in runs of one length.  Splits fill one wave of blocks, a tile for each of a block's four warps at least; where the rows alone fill it, runs of 32 tiles even out
-    ragged batches (64 sequences of up to 8,191 keys, 28 heads of 128 on 4: 57 us, whole sequences 85).  Up to eight splits of one wave join inside a cluster (one
-    sequence of 2,000 keys, 14 heads of 64 on 2: 6.2 us, with a second kernel 7.0; in more waves a cluster waits for its longest split: 82 us for the 57)."""
+    """(rows, n_splits, tiles_per_split, in_cluster) of the form without scratch pages: 8, 16 or 64 rows a block, tiles of 64 keys shared out.
+    Times below are of single tokens, without the projections around them.
+
+    Where the rows leave room for splits in one wave of blocks, each takes an equal share of its sequence (tiles_per_split 0), not a fixed run: `max_kv_len` may be
+    far above the lengths, as a captured decode step's is.  Up to eight splits join inside a cluster, which saves a kernel (one sequence of 2,000 keys, 14 heads of 64 on 2:
+    6.2 us, 7.2 with it).  Up to 64 tiles no more than those eight are made (20 sequences of 2,000: 7.8 us, eleven splits 9.8; 16 of 4,000: 9.8 and 10.0); for longer ones
+    more splits are worth the second kernel (one of 8,000: 10.4 us in eight, 8.6 in 31; 5 of 30,000, 28 heads of 128 on 4: 41 in eight, 32 in 14), of eight tiles at
+    least (one of 32,700, 12 heads of 128 on 2: 13.0 us in 64, 14.0 in 128).
+
+    Where the rows fill the wave, runs of 32 tiles even out ragged batches from 96 tiles on (64 ragged sequences of up to 8,191 keys, 28 heads of 128 on 4: 58 us, whole 78;
+    of up to 6,000: 51 and 57); even ones pay for it there (of 8,191: 101 and 86; of 6,000: 77 and 65), below it both do (of 2,500: 48 and 31, ragged 31 and 27)."""
     group = q_heads // kv_heads
     few = max_q_len * group
     rows = 8 if few <= 8 else 16 if few <= 32 else 64
@@ -1920,12 +1927,16 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
         span = (chunk or window) + tokens + 126
         tiles = min(tiles, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
     wave = n_sms * (3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) // (1 if rows == 8 else 2)
-    splits = wave // blocks
-    per_split = max(4, (-(-tiles // splits) + 3) // 4 * 4) if splits > 1 else 32
-    if tiles < 1.5 * per_split:
+    splits = min(wave // blocks, -(-tiles // 4))
+    if splits > 1:
+        if rows != 64 and tiles <= 64:
+            splits = min(splits, Q8_CLUSTER)
+        elif splits > Q8_CLUSTER:
+            splits = max(Q8_CLUSTER, min(splits, tiles // 8))
+        return rows, splits, 0, rows != 64 and splits <= Q8_CLUSTER
+    if tiles < 96:
         return rows, 1, tiles, False
-    n_splits = -(-tiles // per_split)
-    return rows, n_splits, per_split, rows != 64 and n_splits <= Q8_CLUSTER and blocks * n_splits <= wave
+    return rows, -(-tiles // 32), 32, False
 
 
 Q8_CLUSTER = 8                  # the most key splits that join inside a thread-block cluster, without scratch memory and a second kernel
