@@ -4,8 +4,8 @@
 // The scales are powers of two, so a row's numbers are bfloat16 numbers exactly.  q8_expand_kernel writes the pages that the step's rows
 // see as dense bfloat16 rows once, and the products are those of a bfloat16 cache.  The other places for that conversion were measured and
 // cost more: codes turned into tiles in shared memory by four or eight warps of the attention block itself, anew for every 256 rows
-// (B200, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so, 11 of them the expansion; 4,095 tokens, 14 heads of 64 on 2: 67 and 55, 6 of them:
-// the conversions' instructions and shared-memory traffic hold up the rows and the products alike).
+// (B200, whole calls, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so when the two were compared, 11 of them the expansion; 441 to 459 now, by the GPU;
+// 4,095 tokens, 14 heads of 64 on 2: 67, and 55, 6 of them: the conversions' instructions and shared-memory traffic hold up the rows and the products alike).
 //
 // A block owns 128 rows of one kv head (the group's query heads of 128 / group successive tokens; a row is a token and a head) and walks the
 // keys in tiles of 64, some of them in several hands at once.  Roles:
@@ -17,7 +17,7 @@
 //                  tensor memory, rescaled only when a row's maximum rises by 2^8; at the end the teams' outputs are added.
 // What bounds a tile of 128 x 64: 512 clocks of exponentials, 320 (head size 64) or 640 (128) of products; it takes some 640 and 880, since a row's
 // chain of a tile (scores, maximum, exponentials, probabilities handed over) is 1,900 clocks long and only the teams overlap.  Blocks of 256 rows, a team a
-// row tile, with tiles of 128 keys took 560 and 57 us where these take 469 and 49.
+// row tile, with tiles of 128 keys took 562 and 63 us a call where these took 500 and 55 on that GPU.
 // A sequence's tiles may be shared out over blocks (splits of equal length); q8_combine_kernel joins them.
 //
 // Keys of a missing page are not seen.  Bytes behind the sequence's last key may be anything: scores are replaced, not multiplied, and
@@ -202,8 +202,8 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     auto tile_of = [&](int j) { return j + (j < heads_left ? j0 : shift); };
     const int* pages = a.kv.page_table + (long long)b * a.kv.pages_per_seq;
     auto page_there = [&](int index) { return index < a.kv.pages_per_seq && (unsigned)__ldg(pages + index) < (unsigned)a.kv.n_pages; };
-    // whether every page of the walk is there is found out once: a look at the page list for every tile, by every row's thread, cost a sixth of the
-    // time (2,048 tokens behind 14,000, 28 heads of 128: 467 us, 394 without)
+    // whether every page of the walk is there is found out once, not by every row's thread for every tile (2,048 tokens behind 14,000, 28 heads of 128 on 4, in
+    // turn on one GPU: 458 us, 471 with the look at each tile)
     bool here = true;
     for (int j = threadIdx.x; j < n_tiles; j += X_THREADS) here &= page_there(tile_of(j));
     const bool whole = __syncthreads_and(here);
@@ -323,9 +323,20 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             float sc[X_KEYS];
             tmem_load64(s_addr, sc);
             if (a.cap_over_scale > 0.0f) {
+                // tanh(x) = 1 - 2 / (1 + e^2x), with one reciprocal for four keys: 1/a = b·c·d / (a·b·c·d).  From e^2x = 2^30 on tanh is 1 in float32, so
+                // the product stays below 2^121.  A score that is NaN (its key may be one that the row does not see) is put back and touches no other.
+                // 12 ragged sequences of 600 new tokens, window 1,024, 12 heads of 128: 77 us, 87 with a reciprocal each, 56 uncapped
 #pragma unroll
-                for (int c = 0; c < X_KEYS; ++c)         // tanh(x) = 1 - 2 / (1 + e^2x)
-                    sc[c] = a.cap_over_scale * (1.0f - __fdividef(2.0f, 1.0f + x_exp2(sc[c] * a.cap_exponent)));
+                for (int c = 0; c < X_KEYS; c += 4) {
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = 1.0f + x_exp2(fminf(sc[c + k] * a.cap_exponent, 30.0f));
+                    const float p01 = e[0] * e[1], p23 = e[2] * e[3], r = __fdividef(-2.0f * a.cap_over_scale, p01 * p23);
+                    const float r01 = r * p23, r23 = r * p01;
+                    const float t[4] = {r01 * e[1], r01 * e[0], r23 * e[3], r23 * e[2]};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sc[c + k] = sc[c + k] == sc[c + k] ? a.cap_over_scale + t[k] : sc[c + k];
+                }
             }
             if (masked) {
                 const bool have = whole || page_there(key0 / X_KEYS);

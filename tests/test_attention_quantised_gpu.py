@@ -289,3 +289,35 @@ def test_refusals():
         a = {**ok, **change}
         with pytest.raises(K.KernelError):
             K.attention_quantised(a["q"], a["out"], a["cu"], a["start"], a["n_seqs"], 1, 11, a["H"], a["kv"], a["scale"], **a["more"])
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["keys", "values"])
+@pytest.mark.parametrize("seqs,window", [([(200, 1), (200, 1)], 100), ([(130, 100), (130, 100)], 50)], ids=["single", "chunk"])
+def test_a_capped_score_that_is_not_finite_reaches_no_neighbour(seqs, window, which):
+    """Row 190 of the chunk sees key 141 and not key 140 beside it, which is not finite."""
+    c = Case(14, 2, 64, seqs, seed=31)
+    clean = c.run(window=window, softcap=4.0).view(-1, 14, 64)
+    c.codes[which][1, c.table[0, 2], 1, 12] = 0
+    c.scales[which][1, c.table[0, 2], 1, 12] = 255
+    out = c.run(window=window, softcap=4.0).view(-1, 14, 64)
+    p = torch.arange(seqs[0][0], seqs[0][0] + seqs[0][1], device="cuda")
+    hit = torch.zeros(out.shape[0], 14, dtype=torch.bool, device="cuda")
+    hit[:seqs[0][1], 7:] = ((140 <= p) & (p - 140 < window))[:, None]
+    assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (6, 2, 48)])
+@pytest.mark.parametrize("softcap,size", [(0.5, 40.0), (30.0, 60.0), (2.0, 300.0), (50.0, 0.01)])
+@pytest.mark.parametrize("seqs", [[(150, 1), (63, 1)], [(70, 90), (0, 129)]], ids=["single", "chunk"])
+def test_capped_scores_far_past_the_cap_and_near_zero(H, KV, hd, softcap, size, seqs):
+    c = Case(H, KV, hd, seqs, seed=32, q_size=size)
+    c.check(c.run(softcap=softcap), softcap=softcap)
+
+
+@pytest.mark.parametrize("bound", [2048, 16384, 1 << 20])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("seqs", [[(0, 1)], [(70, 1), (0, 1), (1300, 1)], [(600, 3), (64, 1)]], ids=["one", "three", "few"])
+def test_a_bound_far_above_the_lengths(H, KV, hd, seqs, bound):
+    c = Case(H, KV, hd, seqs, seed=33)
+    c.check(c.run(max_kv=bound))
+    c.check(c.run(max_kv=bound, window=100, keep_first=3, sinks=True), window=100, keep_first=3, sinks=True)
