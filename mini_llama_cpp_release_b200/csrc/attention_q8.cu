@@ -791,14 +791,22 @@ __global__ void __launch_bounds__(Q_THREADS, NT == 1 ? Q_BLOCKS_PER_SM : (Q_BLOC
 // in 32 splits were one chain of loads after another).  A split that saw no key has maximum -inf and sum 0, and its numbers were not written.
 constexpr int Q_JOIN_WARPS = 4;
 __global__ void __launch_bounds__(32 * Q_JOIN_WARPS) q8_combine_kernel(const float* __restrict__ part_ml, const float* __restrict__ part_o, const int* __restrict__ cu_seqlens,
-                                                                       int n_seqs, int n_tokens, int q_heads, int n_splits, const float* __restrict__ sinks,
-                                                                       bf16* __restrict__ out) {
+                                                                       int n_seqs, int n_tokens, int split_tokens, int q_heads, int n_splits,
+                                                                       const float* __restrict__ sinks, bf16* __restrict__ out) {
     constexpr int VECS = Q_HD / 4, PER = (VECS + 31) / 32;          // a lane's pieces of four columns
     __shared__ float4 shares[Q_JOIN_WARPS][VECS];
     grid_launch_dependents();
     grid_dependency_wait();
-    const long long row = blockIdx.x;
-    if (row >= (long long)min(cu_seqlens[n_seqs], n_tokens) * q_heads) return;
+    const long long row = blockIdx.x;              // of the partial results
+    long long out_row = row;
+    if (split_tokens > 0) {                        // the first tokens of every sequence
+        const int token = (int)(row / q_heads), b = token / split_tokens, t = token % split_tokens;
+        const int first = cu_seqlens[b];
+        if (t >= min(cu_seqlens[b + 1], n_tokens) - first) return;
+        out_row = (long long)(first + t) * q_heads + row % q_heads;
+    } else if (row >= (long long)min(cu_seqlens[n_seqs], n_tokens) * q_heads) {
+        return;
+    }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + row * n_splits;
     float all = -INFINITY;
@@ -840,7 +848,7 @@ __global__ void __launch_bounds__(32 * Q_JOIN_WARPS) q8_combine_kernel(const flo
             x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
         const __nv_bfloat162 h0 = __floats2bfloat162_rn(x.x * inv, x.y * inv), h1 = __floats2bfloat162_rn(x.z * inv, x.w * inv);
-        *reinterpret_cast<uint2*>(out + row * Q_HD + 4 * c) = make_uint2(*reinterpret_cast<const unsigned*>(&h0), *reinterpret_cast<const unsigned*>(&h1));
+        *reinterpret_cast<uint2*>(out + out_row * Q_HD + 4 * c) = make_uint2(*reinterpret_cast<const unsigned*>(&h0), *reinterpret_cast<const unsigned*>(&h1));
     }
 }
 
@@ -862,13 +870,13 @@ static cudaError_t shared_memory_of(const void* kernel, int bytes, int which) {
 
 extern "C" int mlc_attention_q8_head_dim() { return Q_HD; }
 
-// Joins n_splits partial results a row (layouts: Q8Args).
-extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_o, const int* cu_seqlens, int n_seqs, int n_tokens, int q_heads,
+// Joins n_splits partial results a row, of every token (split_tokens 0; layouts: Q8Args) or of the first split_tokens of every sequence.
+extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_o, const int* cu_seqlens, int n_seqs, int n_tokens, int split_tokens, int q_heads,
                                         int n_splits, const float* sinks, void* out, void* stream) {
-    const long long blocks = (long long)n_tokens * q_heads;
+    const long long blocks = (split_tokens > 0 ? (long long)n_seqs * split_tokens : n_tokens) * q_heads;
     if (blocks > 0x7fffffffll) return MLC_ERR_BAD_SIZE;
     const cudaError_t e = launch_pdl(q8_combine_kernel, dim3((unsigned)blocks), dim3(32 * Q_JOIN_WARPS), (size_t)0, (cudaStream_t)stream, part_ml, part_o, cu_seqlens,
-                                     n_seqs, n_tokens, q_heads, n_splits, sinks, (bf16*)out);
+                                     n_seqs, n_tokens, split_tokens, q_heads, n_splits, sinks, (bf16*)out);
     return e == cudaSuccess ? 0 : (int)e;
 }
 
@@ -943,5 +951,5 @@ extern "C" int mlc_attention_q8(const void* q, void* out, const int* cu_seqlens,
     }
     e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) return (int)e;
-    return n_splits == 1 || in_cluster ? 0 : mlc_attention_q8_combine(part_ml, part_o, cu_seqlens, n_seqs, n_tokens, q_heads, n_splits, sinks, out, stream);
+    return n_splits == 1 || in_cluster ? 0 : mlc_attention_q8_combine(part_ml, part_o, cu_seqlens, n_seqs, n_tokens, 0, q_heads, n_splits, sinks, out, stream);
 }

@@ -4,7 +4,7 @@
 // The scales are powers of two, so a row's numbers are bfloat16 numbers exactly.  q8_expand_kernel writes the pages that the step's rows
 // see as dense bfloat16 rows once, and the products are those of a bfloat16 cache.  The other places for that conversion were measured and
 // cost more: codes turned into tiles in shared memory by four or eight warps of the attention block itself, anew for every 256 rows
-// (B200, whole calls, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so when the two were compared, 11 of them the expansion; 441 to 459 now, by the GPU;
+// (B200, whole calls, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so when the two were compared, 11 of them the expansion; 404 now;
 // 4,095 tokens, 14 heads of 64 on 2: 67, and 55, 6 of them: the conversions' instructions and shared-memory traffic hold up the rows and the products alike).
 //
 // A block owns 128 rows of one kv head (the group's query heads of 128 / group successive tokens; a row is a token and a head) and walks the
@@ -18,7 +18,7 @@
 // What bounds a tile of 128 x 64: 512 clocks of exponentials, 320 (head size 64) or 640 (128) of products; it takes some 640 and 880, since a row's
 // chain of a tile (scores, maximum, exponentials, probabilities handed over) is 1,900 clocks long and only the teams overlap.  Blocks of 256 rows, a team a
 // row tile, with tiles of 128 keys took 562 and 63 us a call where these took 500 and 55 on that GPU.
-// A sequence's tiles may be shared out over blocks (splits of equal length); q8_combine_kernel joins them.
+// A sequence's first row tiles, which are launched last, may have their keys shared out over blocks in equal parts; q8_combine_kernel joins them.
 //
 // Keys of a missing page are not seen.  Bytes behind the sequence's last key may be anything: scores are replaced, not multiplied, and
 // the expansion writes the values' rows there as zeros.  A key whose key or value row is not finite has NaN for its scores, so that the rows that see it
@@ -52,15 +52,17 @@ struct Q8TcArgs {
     const int* cu_seqlens;
     const int* start_pos;
     QuantisedKV kv;
-    float* part_ml;             // [n_tokens · q_heads][n_splits][2]: maximum (base two), sum
-    float* part_o;              // [n_tokens · q_heads][n_splits][hd], relative to that maximum
+    float* part_ml;             // [sequence][split_tokens][q_heads][n_splits][2]: maximum (base two), sum
+    float* part_o;              // [sequence][split_tokens][q_heads][n_splits][hd], relative to that maximum
     const float* sinks;
     int* status;
     int n_tokens;
     int q_heads, group, heads_per_block, tokens_per_block, head_chunks;
     Q8Mask mask;
     int dense_tiles;            // tiles a sequence has in the expanded keys and values: [sequence][kv head][dense_tiles · 64][hd]
-    int n_splits, tiles_per_split;
+    int row_tiles;              // of the longest sequence
+    int whole_blocks;           // blocks before those that share a row tile's keys out
+    int n_splits, split_tokens; // the first tokens of every sequence are split
     float scale_log2;
     float cap_over_scale, cap_exponent;       // a soft cap c on the scaled scores, as c / scale and 2 log2(e) scale / c (0: none)
 };
@@ -182,11 +184,15 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
     // ---- which rows and which keys; the blocks whose rows see the most keys come first
     const int heads_x = a.kv.kv_heads * a.head_chunks;
-    int at = blockIdx.x;
-    const int split = at % a.n_splits;
-    at /= a.n_splits;
+    const int heads_seq = heads_x * a.kv.n_seqs;
+    const bool parts = (int)blockIdx.x >= a.whole_blocks;
+    int at = parts ? (int)blockIdx.x - a.whole_blocks : (int)blockIdx.x;
+    const int split = parts ? at % a.n_splits : 0;
+    if (parts) at /= a.n_splits;
+    const int row_tile = a.row_tiles - 1 - at / heads_seq - (parts ? a.whole_blocks / heads_seq : 0);
+    at %= heads_seq;
     const int b = at / heads_x, kvh = (at % heads_x) / a.head_chunks, head0 = (at % a.head_chunks) * a.heads_per_block;
-    const int tok0 = (gridDim.y - 1 - blockIdx.y) * a.tokens_per_block;
+    const int tok0 = row_tile * a.tokens_per_block;
     const int seq_tok0 = a.cu_seqlens[b];
     const int q_len = min(a.cu_seqlens[b + 1], a.n_tokens) - seq_tok0;
     const int n_tok = min(a.tokens_per_block, q_len - tok0);                     // <= 0: nothing to do for this block
@@ -196,8 +202,8 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // tiles of kept first keys before the window's first tile are walked ahead of it; behind what a page list holds there are only missing pages
     const int tile_begin = min(a.mask.lowest(p_first) / X_KEYS, a.dense_tiles - 1), head_tiles = min(tile_begin, (keep + X_KEYS - 1) / X_KEYS);
     const int walk = n_tok > 0 ? head_tiles + min(p_last / X_KEYS, a.dense_tiles - 1) + 1 - tile_begin : 0;
-    const int j0 = split * a.tiles_per_split;
-    const int n_tiles = max(0, (split == a.n_splits - 1 ? walk : min(walk, j0 + a.tiles_per_split)) - j0);
+    const int j0 = parts ? (int)((long long)walk * split / a.n_splits) : 0;
+    const int n_tiles = (parts ? (int)((long long)walk * (split + 1) / a.n_splits) : walk) - j0;
     const int heads_left = head_tiles - j0, shift = tile_begin - heads_left;               // (of this block's tiles)
     auto tile_of = [&](int j) { return j + (j < heads_left ? j0 : shift); };
     const int* pages = a.kv.page_table + (long long)b * a.kv.pages_per_seq;
@@ -422,8 +428,8 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             l_all = fmaf(meet[(u * X_ROWS + r) * 2 + 1], f[u], l_all);
         }
         const long long row = (long long)(seq_tok0 + tok0 + t) * a.q_heads + kvh * a.group + hg;
-        const bool parts = a.n_splits > 1;
-        if (parts && row_ok && ok && team == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (row * a.n_splits + split)) = make_float2(m_all, l_all);
+        const long long part = (((long long)b * a.split_tokens + tok0 + t) * a.q_heads + kvh * a.group + hg) * a.n_splits + split;
+        if (parts && row_ok && ok && team == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(m_all, l_all);
         if (a.sinks != nullptr && !parts && row_ok) l_all += x_exp2(a.sinks[kvh * a.group + hg] * 1.4426950408889634f - m_ref);
         // a row that saw no key gives zeros; one that saw a key without a number gives NaN
         const float inv = parts ? 1.0f : m_all == -INFINITY && l_all == l_all ? 0.0f : 1.0f / l_all;
@@ -447,7 +453,7 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             }
             if (row_ok && ok) {
                 if (parts) {
-                    float4* dst = reinterpret_cast<float4*>(a.part_o + (row * a.n_splits + split) * X_HD + 16 * run);
+                    float4* dst = reinterpret_cast<float4*>(a.part_o + part * X_HD + 16 * run);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dst[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
                 } else {
@@ -476,14 +482,16 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
 using namespace mlc;
 
-extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_o, const int* cu_seqlens, int n_seqs, int n_tokens, int q_heads,
+extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_o, const int* cu_seqlens, int n_seqs, int n_tokens, int split_tokens, int q_heads,
                                         int n_splits, const float* sinks, void* out, void* stream);
 
-// As mlc_attention_q8, for head sizes of 64 and 128 (others are refused): 128 rows a block, tiles_per_split in tiles of 64 keys.  dense: scratch of
+// As mlc_attention_q8, for head sizes of 64 and 128 (others are refused): 128 rows a block.  The keys of the last split_tiles row tiles to be
+// launched (every sequence's first ones) are shared out over n_splits blocks each; those need part_ml and part_o (layouts: Q8TcArgs, split_tokens = split_tiles ·
+// tokens of a block).  dense: scratch of
 // 2 · n_seqs · kv_heads · dense_tiles · 64 · head_dim bfloat16, with at least as many tiles as pages_per_seq (and one).
 extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_seqlens, const int* start_pos, int n_seqs, int n_tokens, int max_q_len,
                                         int q_heads, int kv_heads, int hd, float scale, int window, int keep_first, int chunk, float softcap,
-                                        const float* sinks, int n_splits, int tiles_per_split, float* part_ml, float* part_o, void* dense, int dense_tiles,
+                                        const float* sinks, int n_splits, int split_tiles, float* part_ml, float* part_o, void* dense, int dense_tiles,
                                         void* k_pool, void* v_pool, void* k_scale, void* v_scale, const int* page_table, int n_lists, int pages_per_seq,
                                         long long entry_offset, long long n_pages, int page_size, int* status, void* stream) {
 #if MLC_Q8_TCGEN05
@@ -491,7 +499,7 @@ extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_
     if (chunk < 0 || (chunk > 0 && window > 0) || !(softcap >= 0.0f)) return MLC_ERR_UNSUPPORTED;
     if (n_seqs <= 0 || n_tokens <= 0 || max_q_len <= 0) return 0;
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || status == nullptr || n_pages <= 0 || n_pages > 0x7fffffffll || pages_per_seq < 0 || n_lists < n_seqs) return MLC_ERR_BAD_SIZE;
-    if (!(scale > 0.0f) || window < 0 || n_splits < 1 || tiles_per_split < 1) return MLC_ERR_BAD_SIZE;
+    if (!(scale > 0.0f) || window < 0 || n_splits < 1 || split_tiles < 0 || (n_splits > 1) != (split_tiles > 0)) return MLC_ERR_BAD_SIZE;
     if (n_splits > 1 && (part_ml == nullptr || part_o == nullptr)) return MLC_ERR_BAD_SIZE;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)dense) & 15) return MLC_ERR_BAD_SIZE;
     if (entry_offset < 0 || entry_offset % ((long long)hd * X_KEYS) != 0) return MLC_ERR_BAD_SIZE;
@@ -516,14 +524,17 @@ extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_
     a.head_chunks = (a.group + a.heads_per_block - 1) / a.heads_per_block;
     a.mask = Q8Mask{window, keep_first < 0 ? 0 : keep_first, chunk};
     a.dense_tiles = dense_tiles;
-    a.n_splits = n_splits;
-    a.tiles_per_split = tiles_per_split;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.cap_over_scale = softcap > 0.0f ? softcap / scale : 0.0f;
     a.cap_exponent = softcap > 0.0f ? 2.0f * 1.4426950408889634f * scale / softcap : 0.0f;
-    const long long blocks = (long long)n_splits * kv_heads * a.head_chunks * n_seqs;
-    const int tiles_y = (max_q_len + a.tokens_per_block - 1) / a.tokens_per_block;
-    if (blocks > 0x7fffffffll || tiles_y > 65535) return MLC_ERR_BAD_SIZE;
+    a.row_tiles = (max_q_len + a.tokens_per_block - 1) / a.tokens_per_block;
+    if (split_tiles > a.row_tiles) return MLC_ERR_BAD_SIZE;
+    const long long heads_seq = (long long)kv_heads * a.head_chunks * n_seqs, whole_blocks = heads_seq * (a.row_tiles - split_tiles);
+    const long long blocks = whole_blocks + heads_seq * split_tiles * n_splits;
+    if (blocks > 0x7fffffffll) return MLC_ERR_BAD_SIZE;
+    a.whole_blocks = (int)whole_blocks;
+    a.n_splits = n_splits;
+    a.split_tokens = split_tiles * a.tokens_per_block;
     bf16* k_dense = (bf16*)dense;
     bf16* v_dense = k_dense + dense_rows * hd;
     CUtensorMap map_q, map_k, map_v;
@@ -554,9 +565,9 @@ extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_
     e = launch_pdl(q8_expand_kernel, dim3(dense_tiles, kv_heads, n_seqs), dim3(XE_THREADS), (size_t)0, (cudaStream_t)stream, a.kv, cu_seqlens, start_pos, n_tokens,
                    a.mask, dense_tiles, k_dense, v_dense);
     if (e != cudaSuccess) return (int)e;
-    e = launch_pdl(attention_q8_tcgen05_kernel, dim3((unsigned)blocks, tiles_y), dim3(X_THREADS), (size_t)X_SMEM_BYTES, (cudaStream_t)stream, map_q, map_k, map_v, a);
+    e = launch_pdl(attention_q8_tcgen05_kernel, dim3((unsigned)blocks), dim3(X_THREADS), (size_t)X_SMEM_BYTES, (cudaStream_t)stream, map_q, map_k, map_v, a);
     if (e != cudaSuccess) return (int)e;
-    return n_splits == 1 ? 0 : mlc_attention_q8_combine(part_ml, part_o, cu_seqlens, n_seqs, n_tokens, q_heads, n_splits, sinks, out, stream);
+    return n_splits == 1 ? 0 : mlc_attention_q8_combine(part_ml, part_o, cu_seqlens, n_seqs, n_tokens, a.split_tokens, q_heads, n_splits, sinks, out, stream);
 #else
     return MLC_ERR_UNSUPPORTED;
 #endif

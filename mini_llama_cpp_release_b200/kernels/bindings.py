@@ -1955,22 +1955,32 @@ def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
 
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
-    """(n_splits, tiles_per_split) of the form with 128 rows a block, or None where it is not for these sizes."""
+    """(n_splits, split_tiles) of the form with 128 rows a block, or None where it is not for these sizes: the keys of every sequence's first `split_tiles`
+    row tiles are shared out over n_splits blocks."""
     group = q_heads // kv_heads
     if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len < 2 or max_q_len * group < 64:
         return None
     heads = min(group, 128)
     tokens = 128 // heads
-    blocks = ((max_q_len + tokens - 1) // tokens) * kv_heads * ((group + heads - 1) // heads) * n_seqs
+    row_tiles = (max_q_len + tokens - 1) // tokens
+    across = kv_heads * ((group + heads - 1) // heads) * n_seqs
     longest = (max_kv_len + 63) // 64
     if window or chunk:
-        span = (chunk or window) + tokens + 126
-        longest = min(longest, span // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
-    # a key range is shared out only to fill the first wave of blocks: the joining costs what it saves from there on (one prompt of 4,095 tokens, 14 heads
-    # of 64 on 2, 228 blocks: 55 us, in two splits 83)
-    wanted = max(1, n_sms // blocks)
-    per_split = max(8, (longest + wanted - 1) // wanted)
-    return (longest + per_split - 1) // per_split, per_split
+        longest = min(longest, ((chunk or window) + tokens + 126) // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
+    # Blocks run in whole waves, and what is left over would take as long as a full one: its keys are shared out where that is sooner.  In tiles: a block's start and
+    # end are eight, the joining twelve, 0.3 a block's rows and 0.1 their share of a split (512 new behind 20,000, 28 heads of 128 on 4, 116 blocks: 156 us, in two
+    # splits 186; 2,048 behind 14,000, 456 blocks, 12 of them in twelve splits each: 404 us, 451 without; behind 30,000: 811 and 927; 100 behind 30,000, 14 heads of 64 on 2,
+    # 12 blocks: 31 and 172).  Behind full waves only for one sequence: the lengths of several are not known here.
+    split_tiles = row_tiles - row_tiles * across // n_sms * n_sms // across
+    left = split_tiles * across
+    length = longest
+    if left < row_tiles * across:
+        length = min(longest, (max(0, max_kv_len - max_q_len) + split_tiles * tokens + 63) // 64)
+        if n_seqs > 1 or left == 0:
+            return 1, 0
+    n_splits = min(range(1, max(16, n_sms // left) + 1),
+                   key=lambda n: -(-left * n // n_sms) * (length / n + 8) + (12 + 0.3 * left + 0.1 * left * n if n > 1 else 0))
+    return (n_splits, split_tiles) if n_splits > 1 else (1, 0)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2018,22 +2028,24 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
         dense = _spare_rows(n_seqs * kv.kv_heads * dense_tiles * 128 * kv.head_dim, q.device)
         if dense is None:
             form = attention_q8_plan(*sizes)
+    part_tokens = n
     if dense is not None:
-        (n_splits, per_split), in_cluster = form, False
+        (n_splits, split_tiles), in_cluster = form, False
+        part_tokens = n_seqs * split_tiles * (128 // min(q_heads // kv.kv_heads, 128))
     else:
         rows, n_splits, per_split, in_cluster = form
     part_ml = part_o = None
     joined_later = n_splits > 1 and not in_cluster
     if joined_later:
-        part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
-        part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(part_tokens * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
+        part_o = torch.empty(part_tokens * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
     status = _status.get(device)
     if status is None:
         status = gemm_status(q.device)
     head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, scale, window,
             keep_first, chunk, softcap, _ptr(sinks))
     if dense is not None:
-        rc = lib.mlc_attention_q8_tcgen05(*head, n_splits, per_split, _ptr(part_ml), _ptr(part_o), dense.data_ptr(), dense_tiles, *args, status.data_ptr(), _stream())
+        rc = lib.mlc_attention_q8_tcgen05(*head, n_splits, split_tiles, _ptr(part_ml), _ptr(part_o), dense.data_ptr(), dense_tiles, *args, status.data_ptr(), _stream())
         count_launches(1)
     else:
         rc = lib.mlc_attention_q8(*head, rows, n_splits, per_split, _ptr(part_ml), _ptr(part_o), *args, status.data_ptr(), _stream())

@@ -321,3 +321,35 @@ def test_a_bound_far_above_the_lengths(H, KV, hd, seqs, bound):
     c = Case(H, KV, hd, seqs, seed=33)
     c.check(c.run(max_kv=bound))
     c.check(c.run(max_kv=bound, window=100, keep_first=3, sinks=True), window=100, keep_first=3, sinks=True)
+
+
+@pytest.mark.parametrize("n_splits,split_tiles", [(2, 1), (5, 3), (16, 8)])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("mask", [dict(), dict(sinks=True, softcap=5.0), dict(window=70, keep_first=65, sinks=True), dict(chunk=100)],
+                         ids=["all", "sinks", "window", "chunk"])
+def test_first_row_tiles_shared_out_and_the_others_whole(monkeypatch, H, KV, hd, n_splits, split_tiles, mask):
+    """Sequences shorter than the split rows, one without new tokens, a page that is missing, and rows behind the last sequence's."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    monkeypatch.setattr(bindings, "_attention_q8_form", lambda *sizes: (n_splits, min(split_tiles, -(-150 // (128 // (H // KV))))))
+    empty = torch.empty
+
+    def spoilt(*a, **k):
+        t = empty(*a, **k)
+        return t.fill_(float("nan")) if t.is_floating_point() else t
+
+    monkeypatch.setattr(bindings.torch, "empty", spoilt)
+    c = Case(H, KV, hd, [(70, 90), (0, 150), (500, 3), (10, 0), (700, 20)], seed=34, tail=3)
+    c.check(c.run(**mask), **mask)
+    table = c.table.clone()
+    table[0, 0] = table[4, 3] = -1
+    c.check(c.run(table=table, **mask), gone=[(0, 0), (4, 3)], **mask)
+
+
+@pytest.mark.parametrize("H,KV,hd,new,cached", [(28, 4, 128, 700, 3000), (14, 2, 64, 1400, 9000)])
+def test_a_partial_wave_behind_whole_ones(H, KV, hd, new, cached):
+    plan = kernels().attention_q8_tcgen05_plan(new, 1, new + cached, H, KV, hd, torch.cuda.get_device_properties(0).multi_processor_count)
+    assert plan[0] > 1 and 0 < plan[1] < -(-new // (128 // (H // KV)))
+    c = Case(H, KV, hd, [(cached, new)], seed=35, tail=1)
+    c.check(c.run())
+    again = c.run()
+    assert torch.equal(again, c.run())

@@ -75,7 +75,7 @@ def test_plans_cover_every_key():
                         assert per == 0 or n * per >= tiles or mask, (q_len, seqs, keys)
                         assert not cluster or (1 < n <= 8 and rows != 64)
                         p = attention_q8_tcgen05_plan(q_len, seqs, max(keys, q_len), heads, kv_heads, hd, 148, **mask)
-                        assert p is None or p[0] >= 1 and (p[0] * p[1] >= tiles or mask)
+                        assert p is None or p[0] >= 1 and (p[0] > 1) == (p[1] > 0) and p[1] <= q_len
 
 
 def test_the_plain_form_of_the_format():
