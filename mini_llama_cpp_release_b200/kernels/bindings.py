@@ -1869,7 +1869,8 @@ def quantise_kv(k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Ten
     """The rows k, v [tokens, kv_heads, head_dim] (float32 or bfloat16; token and head strides are free) into the cache, each
     row's numbers in e4m3 beside the smallest power of two 2^e, -100 <= e <= 119, with max|x| <= 448 · 2^e (a larger row saturates; a row
     with an infinity or a NaN reads as NaN).  Token i belongs at position positions[i] of sequence tok_seq[i]; one whose page is
-    missing is left out.  `v` is None for an entry whose values are its key rows."""
+    missing is left out.  `v` is None for an entry whose values are its key rows.  No two tokens of a call have one place: their rows are written side
+    by side, and what is left there would be numbers of one beside the scale of the other."""
     args = _quantised_rows("quantise_kv", k, v, positions, tok_seq, kv)
     if k.shape[0]:
         _check(core().mlc_quantise_kv(*args), "cache quantisation")
@@ -1914,8 +1915,11 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
     more splits are worth the second kernel (one of 8,000: 10.4 us in eight, 8.6 in 31; 5 of 30,000, 28 heads of 128 on 4: 41 in eight, 32 in 14), of eight tiles at
     least (one of 32,700, 12 heads of 128 on 2: 13.0 us in 64, 14.0 in 128).
 
-    Where the rows fill the wave, runs of 32 tiles even out ragged batches from 96 tiles on (64 ragged sequences of up to 8,191 keys, 28 heads of 128 on 4: 58 us, whole 78;
-    of up to 6,000: 51 and 57); even ones pay for it there (of 8,191: 101 and 86; of 6,000: 77 and 65), below it both do (of 2,500: 48 and 31, ragged 31 and 27)."""
+    Where the rows fill one wave and not two, runs of 32 tiles even out ragged batches from 96 tiles on (64 ragged sequences of up to 8,191 keys, 28 heads of 128 on 4: 58 us,
+    whole 78; of up to 6,000: 51 and 57); even ones pay for it there (of 8,191: 101 and 86; of 6,000: 77 and 65), below it both do (of 2,500: 48 and 31, ragged 31 and 27),
+    and from two waves on too (256 sequences of 7,000: 327 and 289, ragged 184 and 171; 128: ragged 99 and 109).  64 rows: two equal shares up to four waves (1,000 behind 7,000,
+    12 heads of 48 on 4: 199 us, whole 361, runs of 32 208; 3,000: 595, 737, 610; 8 heads of 256 on 1, 1,000: 550, 565, 569, and 2,000: 1,145, 1,116, 1,101).  The limits also
+    bound the partial results, which 16,384 tokens behind 84,000 with 32 heads of 256 would have made 24 GB."""
     group = q_heads // kv_heads
     few = max_q_len * group
     rows = 8 if few <= 8 else 16 if few <= 32 else 64
@@ -1934,9 +1938,12 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
         elif splits > Q8_CLUSTER:
             splits = max(Q8_CLUSTER, min(splits, tiles // 8))
         return rows, splits, 0, rows != 64 and splits <= Q8_CLUSTER
-    if tiles < 96:
+    if tiles < 96 or blocks >= (4 if rows == 64 else 2) * wave:
         return rows, 1, tiles, False
-    return rows, -(-tiles // 32), 32, False
+    if rows == 64:
+        return rows, 2, 0, False
+    run = max(32, -(-tiles // 64))
+    return rows, -(-tiles // run), run, False
 
 
 Q8_CLUSTER = 8                  # the most key splits that join inside a thread-block cluster, without scratch memory and a second kernel

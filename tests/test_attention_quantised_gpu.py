@@ -353,3 +353,13 @@ def test_a_partial_wave_behind_whole_ones(H, KV, hd, new, cached):
     c.check(c.run())
     again = c.run()
     assert torch.equal(again, c.run())
+
+
+@pytest.mark.parametrize("H,KV,hd,seqs", [(12, 4, 48, [(6000, 300)]), (8, 1, 256, [(6100, 140), (20, 200)])], ids=["48", "256"])
+def test_long_chunks_of_other_head_sizes_in_two_shares(H, KV, hd, seqs):
+    plan = kernels().attention_q8_plan(max(n for _, n in seqs), len(seqs), max(c + n for c, n in seqs), H, KV, hd,
+                                       torch.cuda.get_device_properties(0).multi_processor_count)
+    assert plan[0] == 64 and plan[1] >= 2
+    c = Case(H, KV, hd, seqs, seed=36, tail=1)
+    c.check(c.run())
+    c.check(c.run(sinks=True, softcap=9.0), sinks=True, softcap=9.0)

@@ -116,3 +116,16 @@ def test_argument_lists_are_the_kernels():
         for a in (x.strip() for x in declared.split(",")):
             got += bindings.QUANTISED_ARGS if a == "*QUANTISED_ARGS" else [names[a]]
         assert got == want, entry
+
+
+def test_partial_results_stay_small():
+    """Whatever the sizes and however far a bound lies above the lengths, splits that a second kernel joins need no more than 2 GiB."""
+    for heads, kv_heads, hd in ((14, 2, 64), (28, 4, 128), (12, 4, 48), (32, 4, 256), (64, 8, 128), (8, 8, 16)):
+        for q_len, seqs, keys in ((1, 1, 1 << 20), (1, 400, 1 << 20), (1, 4000, 65536), (3, 64, 200000), (16384, 1, 100000), (8192, 1, 30000), (1024, 16, 16000),
+                                  (300, 2, 1 << 20), (40, 1, 1 << 20)):
+            rows, n, per, cluster = attention_q8_plan(q_len, seqs, keys, heads, kv_heads, hd, 148)
+            if n > 1 and not cluster:
+                assert q_len * seqs * heads * n * (hd + 2) * 4 <= 2 << 30, (heads, hd, q_len, seqs, keys, n)
+            p = attention_q8_tcgen05_plan(q_len, seqs, keys, heads, kv_heads, hd, 148)
+            if p is not None and p[0] > 1:
+                assert seqs * p[1] * (128 // min(heads // kv_heads, 128)) * heads * p[0] * (hd + 2) * 4 <= 2 << 30, (heads, hd, q_len, seqs, keys, p)
