@@ -64,8 +64,8 @@ def padded_batch(n: int) -> int:
 class DecodeRunner:
     """Buffers and graph for `n_seqs` rows decoding together, valid while no sequence grows beyond `max_len` tokens.
     A batch of fewer sequences fills the remaining rows with copies of its last one: a copy computes the same
-    values from the same inputs and writes the same keys and values to the same places, so it changes no result; its
-    chosen token is dropped.  (A mixer that keeps state could not tell a copy from a second step, so models with
+    values from the same inputs and writes the same keys and values to the same places (to an 8-bit cache none), so it changes no
+    result; its chosen token is dropped.  (A mixer that keeps state could not tell a copy from a second step, so models with
     state get a runner of the batch's exact size.)  The sampler's seed stands in the buffer, not in the graph."""
 
     HISTORY_STEPS = 1024
@@ -84,7 +84,7 @@ class DecodeRunner:
         n_groups = len(self.cache.groups)
         # one int32 buffer; the per-step inputs come first so that one copy brings them
         inputs = ["tokens", "positions", "start_pos", "sample_pos"] + (["row_seq"] if self.cache.quantised else [])
-        names = [(name, B) for name in inputs] + [("row_index", B)] * self.cache.quantised + [
+        names = [(name, B) for name in inputs] + [("row_index", B), ("store_seq", B)] * self.cache.quantised + [
                  ("tok_seq", B), ("cu_seqlens", B + 1), ("slots", B), ("want_rows", B), ("seq_ids", B), ("chosen", B),
                  ("counter", 1), ("seed", 2)] + [(f"pages{g}", B * self.pages_per_seq) for g in range(n_groups)]
         self.offsets = {}
@@ -146,7 +146,8 @@ class DecodeRunner:
                         tokens=self.view("tokens"), positions=self.view("positions"), tok_seq=self.view("tok_seq"),
                         cu_seqlens=self.view("cu_seqlens"), start_pos=self.view("start_pos"), slots=self.view("slots"),
                         want_rows=self.view("want_rows"), page_tables=tables, slots_long=self.slots_long, wants_every_row=True,
-                        token_rows=(self.view("row_index").view(B, 1), self.view("row_seq")) if self.cache.quantised else None)
+                        token_rows=(self.view("row_index").view(B, 1), self.view("row_seq")) if self.cache.quantised else None,
+                        store_seq=self.view("store_seq") if self.cache.quantised else None)
 
     # ------------------------------------------------------------------ one step's body
     def _body(self) -> None:
@@ -202,6 +203,9 @@ class DecodeRunner:
         h("sample_pos")[:] = h("positions") + 1
         if self.cache.quantised:
             h("row_seq")[:] = h("row_index") - h("positions")
+            # a copy's sums may differ from its original's in their last bits: its codes beside the other's scale would be another row
+            h("store_seq")[:] = h("tok_seq")
+            h("store_seq")[self.n_live:] = -1
         h("slots")[:] = torch.tensor(list(slots), dtype=torch.int32)
         h("seq_ids")[:] = torch.tensor(list(seq_ids), dtype=torch.int32)
         h("counter")[:] = 0

@@ -34,6 +34,8 @@ class StepInfo:
     # sequence · pages a list + its position), so lists of one page and t - position for the sequence lead to t.  Part of the
     # description, which is complete before a step's first kernel: some of those kernels read it ahead of what runs before them.
     token_rows: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+    # `tok_seq` for writing to an 8-bit cache, where it differs: -1 for a spare row, a copy of another that has its place (None: `tok_seq`)
+    store_seq: Optional[torch.Tensor] = None
     wants_every_row: bool = False     # known to the host: `want_rows` is 0, 1, ..., n_tokens - 1
     # what one part leaves for the next part of the same step (a block that has just written the residual stream's
     # 16-bit copy hands it to the block that reads it); keyed by the leaving part's choice, gone with the step

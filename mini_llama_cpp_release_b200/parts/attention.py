@@ -137,7 +137,7 @@ class GQAttention(Part):
         if place is not None and place is not memory.kv:
             k = place.k_pool.view(step.n_tokens, place.kv_heads, place.head_dim)
             v = None if place.v_pool is place.k_pool else place.v_pool.view(step.n_tokens, place.kv_heads, place.head_dim)
-            kernels.quantise_kv(k, v, step.positions, step.tok_seq, memory.kv)
+            kernels.quantise_kv(k, v, step.positions, step.tok_seq if step.store_seq is None else step.store_seq, memory.kv)
 
     def forward(self, h, step, memory: MixerMemory, residual: Optional[torch.Tensor] = None):
         rt = self.runtime

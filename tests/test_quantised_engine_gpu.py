@@ -191,3 +191,30 @@ def test_refusals():
         Context(llm.model, 1024, cache_dtype="float8_e4m3")
     with pytest.raises(ValueError, match="pages of 64"):
         Context(ml.load(folder("A")).model, 1024, page_size=32, cache_dtype="float8_e4m3")
+
+
+@pytest.mark.parametrize("n", [5, 3, 7])
+def test_no_row_of_the_cache_is_written_twice_in_a_step(n, monkeypatch):
+    """A captured step is made for a few batch sizes and fills its spare rows with copies of the last sequence.  A copy's sums may differ in
+    their last bits, and its codes beside the other's scale would be another row."""
+    import mini_llama_cpp_release_b200.kernels as kernels
+    calls = []
+    quantise = kernels.quantise_kv
+
+    def spy(k, v, positions, tok_seq, kv):
+        calls.append((positions, tok_seq, kv.page_table))
+        quantise(k, v, positions, tok_seq, kv)
+
+    monkeypatch.setattr(kernels, "quantise_kv", spy)
+    ctx = ml.load(folder("C"), max_tokens=2048, cache_dtype="float8_e4m3").context
+    slots = [ctx.acquire() for _ in range(n)]
+    ctx.forward_batch(MiniBatch.prefill(slots, [helpers.random_tokens(10 + i, 777, 80 + i) for i in range(n)]))
+    sampler = DeviceSampler(SamplingParams(), ctx.model.runtime.device)
+    ctx.decode_and_sample(slots, list(range(n)), sampler, list(range(n)))
+    for live in (n, n - 1):                         # the second in the same captured step, where there is one
+        ctx.decode_and_sample(slots[:live], list(range(live)), sampler, list(range(live)))
+        torch.cuda.synchronize()
+        for positions, tok_seq, table in calls:
+            places = [(int(table[s, p // 64]), int(p) % 64) for p, s in zip(positions.tolist(), tok_seq.tolist()) if s >= 0]
+            assert len(set(places)) == len(places)
+    assert any(t.shape[0] > n - 1 for _, t, _ in calls[2:])
