@@ -363,3 +363,39 @@ def test_long_chunks_of_other_head_sizes_in_two_shares(H, KV, hd, seqs):
     c = Case(H, KV, hd, seqs, seed=36, tail=1)
     c.check(c.run())
     c.check(c.run(sinks=True, softcap=9.0), sinks=True, softcap=9.0)
+
+
+@pytest.mark.parametrize("form", [(5, 3), (8, 0, "few")], ids=["first row tiles", "equal shares"])
+def test_two_captured_graphs_with_splits_and_other_lengths_at_replay(monkeypatch, form):
+    """Partial results are each graph's own, and shares follow the lengths that the replay finds."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    seqs = [(70, 90), (500, 130)] if len(form) == 2 else [(700, 1), (90, 1), (1500, 1)]
+    monkeypatch.setattr(bindings, "_attention_q8_form", lambda *sizes: form if len(form) == 2 else (8, 8, 0, False))
+    cases = [Case(14, 2, 64, seqs, seed=40 + i, tail=1) for i in range(2)]
+    streams, graphs, outs, views = [torch.cuda.Stream() for _ in cases], [], [torch.full_like(c.q, 7.0) for c in cases], [c.view() for c in cases]
+
+    def call(i):
+        c = cases[i]
+        kernels().attention_quantised(c.q, outs[i], c.cu, c.start, len(seqs), max(n for _, n in seqs), 4096, 14, views[i], 0.125)
+
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call(i)
+        s.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=s):
+            call(i)
+    for cut in (0, 33, 37):
+        for i, c in enumerate(cases):
+            c.start -= cut
+            c.seqs = [(cached - cut, n) for cached, n in c.seqs]
+            c.k, c.v = [k[:len(k) - cut] for k in c.k], [v[:len(v) - cut] for v in c.v]
+            outs[i].fill_(7.0)
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i, c in enumerate(cases):
+            c.check(outs[i])
