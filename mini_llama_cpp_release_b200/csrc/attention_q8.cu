@@ -744,6 +744,7 @@ __global__ void __launch_bounds__(Q_THREADS, NT == 1 ? Q_BLOCKS_PER_SM : (Q_BLOC
             *reinterpret_cast<float4*>(share + r * Q_HD + col) = v;
             if (col == 0) *reinterpret_cast<float2*>(share_ml + 2 * r) = make_float2(all, fine_here ? sum : -1.0f);      // (-1: a wait ran out)
         }
+        __syncwarp();                                                      // the lanes went round the loop apart, and the cluster's barrier takes whole warps
         cluster_sync_all();
         for (int u = threadIdx.x + 32 * Q_WARPS * k.split; u < ROWS * (Q_HD / 4); u += 32 * Q_WARPS * a.n_splits) {
             const int r = u / (Q_HD / 4), col = u % (Q_HD / 4) * 4, tk = r / a.heads_per_block, hg = k.head0 + r % a.heads_per_block;
@@ -766,6 +767,7 @@ __global__ void __launch_bounds__(Q_THREADS, NT == 1 ? Q_BLOCKS_PER_SM : (Q_BLOC
             const float value[4] = {v.x, v.y, v.z, v.w};
             if (good) q8_finish(a, row, all, sum, [&](int i) { return value[i]; }, col, 4);
         }
+        __syncwarp();
         cluster_sync_all();                                                // a block's shared memory stays until the others have read it
         return;
     }

@@ -129,3 +129,14 @@ def test_partial_results_stay_small():
             p = attention_q8_tcgen05_plan(q_len, seqs, keys, heads, kv_heads, hd, 148)
             if p is not None and p[0] > 1:
                 assert seqs * p[1] * (128 // min(heads // kv_heads, 128)) * heads * p[0] * (hd + 2) * 4 <= 2 << 30, (heads, hd, q_len, seqs, keys, p)
+
+
+def test_warps_come_whole_to_the_clusters_barriers():
+    """`barrier.cluster` in its aligned form is for whole warps: behind a loop that lanes leave one by one they are brought together first."""
+    import os
+    import re
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    with open(os.path.join(os.path.dirname(bindings._build.__file__), "attention_q8.cu")) as f:
+        code = [line for line in (re.sub(r"//.*", "", x).strip() for x in f) if line]
+    before = [code[i - 1] for i, line in enumerate(code) if line == "cluster_sync_all();"]
+    assert len(before) == 2 and all(line == "__syncwarp();" for line in before)
