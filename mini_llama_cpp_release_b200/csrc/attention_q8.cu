@@ -806,8 +806,8 @@ __global__ void __launch_bounds__(32 * Q_JOIN_WARPS) q8_combine_kernel(const flo
         const int first = cu_seqlens[b];
         if (t >= min(cu_seqlens[b + 1], n_tokens) - first) return;
         out_row = (long long)(first + t) * q_heads + row % q_heads;
-    } else if (row >= (long long)min(cu_seqlens[n_seqs], n_tokens) * q_heads) {
-        return;
+    } else if (row < (long long)cu_seqlens[0] * q_heads || row >= (long long)min(cu_seqlens[n_seqs], n_tokens) * q_heads) {
+        return;                                    // no sequence's: left as it is
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + row * n_splits;

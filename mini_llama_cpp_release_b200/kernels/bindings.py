@@ -2002,8 +2002,8 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     """Attention of bfloat16 q [tokens, q_heads · head_dim] over an 8-bit cache entry, into `out` of the same shape: tokens
     cu_seqlens[b] ... cu_seqlens[b + 1] are sequence b's, the first of them at position start_pos[b]; the entry holds their own keys already.
     `max_q_len`, `max_kv_len`: bounds of a sequence's new tokens and of its keys with them.  `window`, `sinks`, `keep_first`, `chunk` and
-    `softcap` as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows behind the
-    last sequence's are left as they are."""
+    `softcap` as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows before the
+    first sequence's and behind the last one's are left as they are."""
     device = kv.check()
     _on_device(device, q, out, cu_seqlens, start_pos, sinks)
     n = q.shape[0]

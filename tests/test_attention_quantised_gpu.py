@@ -399,3 +399,21 @@ def test_two_captured_graphs_with_splits_and_other_lengths_at_replay(monkeypatch
         torch.cuda.synchronize()
         for i, c in enumerate(cases):
             c.check(outs[i])
+
+
+@pytest.mark.parametrize("form", [(8, 5, 0, False), (8, 4, 0, True), (8, 3, 5, False), (64, 2, 0, False), (3, 1), (1, 0)], ids=str)
+def test_rows_before_the_first_sequence_are_left_as_they_are(monkeypatch, form):
+    """Whatever lies in fresh memory, the joining of key splits writes the sequences' rows only."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    monkeypatch.setattr(bindings, "_attention_q8_form", lambda *sizes: form)
+    empty = torch.empty
+    monkeypatch.setattr(bindings.torch, "empty", lambda *a, **k: (lambda t: t.fill_(3.0) if t.is_floating_point() else t)(empty(*a, **k)))
+    c = Case(14, 2, 64, [(900, 1), (70, 1)] if form[0] == 8 else [(900, 9), (70, 2)], seed=50, tail=2)
+    before = 3
+    q, cu = c.q, c.cu
+    c.q = torch.cat([q[:before], q])
+    c.cu = cu + before
+    out = c.run()
+    assert (out[:before] == 7.0).all()
+    c.q, c.cu = q, cu
+    c.check(out[before:])
