@@ -1946,6 +1946,10 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
     return rows, -(-tiles // run), run, False
 
 
+# The largest soft cap c.  The kernels compute c · (1 - 2 / (1 + e^2y)) in float32.  The quotient q is 2 at most; two units of a fast division are 2^-22, the exponential's
+# and the sum's roundings 2^-24 of q each, the difference's 2^-24: a score is off by less than c · 2^-21.  At 2,048 that is 2^-10, and what it moves a weight by comes up to
+# the half step to which the result is rounded.
+Q8_LARGEST_CAP = 2048.0
 Q8_CLUSTER = 8                  # the most key splits that join inside a thread-block cluster, without scratch memory and a second kernel
 EXPANDED_BYTES = 8 << 30        # the most scratch memory for pages written out as bfloat16 (a call that would want more runs in the form without)
 
@@ -2002,8 +2006,11 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     """Attention of bfloat16 q [tokens, q_heads · head_dim] over an 8-bit cache entry, into `out` of the same shape: tokens
     cu_seqlens[b] ... cu_seqlens[b + 1] are sequence b's, the first of them at position start_pos[b]; the entry holds their own keys already.
     `max_q_len`, `max_kv_len`: bounds of a sequence's new tokens and of its keys with them.  `window`, `sinks`, `keep_first`, `chunk` and
-    `softcap` as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows before the
+    `softcap` (at most `Q8_LARGEST_CAP`) as for `attention_simt`.  Keys of a missing page are not seen, a row that sees none gives zeros, and rows before the
     first sequence's and behind the last one's are left as they are."""
+    if not 0 < scale < float("inf") or window < 0 or keep_first < 0 or chunk < 0 or not 0 <= softcap <= Q8_LARGEST_CAP or (window and chunk):
+        raise KernelError(f"attention over an 8-bit cache: scale {scale}, window {window}, keep_first {keep_first}, chunk {chunk}, softcap {softcap} "
+                          f"(at most {Q8_LARGEST_CAP})")
     device = kv.check()
     _on_device(device, q, out, cu_seqlens, start_pos, sinks)
     n = q.shape[0]
@@ -2020,8 +2027,6 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     if kv.page_size != 64 or kv.page_table.shape[0] < n_seqs:
         raise KernelError(f"attention over an 8-bit cache: pages of 64 tokens and a page list per sequence, got pages of {kv.page_size} and "
                           f"{kv.page_table.shape[0]} lists for {n_seqs}")
-    if not scale > 0 or window < 0 or keep_first < 0 or chunk < 0 or not softcap >= 0 or (window and chunk):
-        raise KernelError(f"attention over an 8-bit cache: scale {scale}, window {window}, keep_first {keep_first}, chunk {chunk}, softcap {softcap}")
     if n == 0 or n_seqs <= 0 or max_q_len <= 0:
         return
     lib = _attn_q8_libs.get(kv.head_dim) or attention_q8_library(kv.head_dim)

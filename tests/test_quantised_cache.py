@@ -140,3 +140,32 @@ def test_warps_come_whole_to_the_clusters_barriers():
         code = [line for line in (re.sub(r"//.*", "", x).strip() for x in f) if line]
     before = [code[i - 1] for i, line in enumerate(code) if line == "cluster_sync_all();"]
     assert len(before) == 2 and all(line == "__syncwarp();" for line in before)
+
+
+@pytest.mark.parametrize("bad", [dict(scale=math.inf), dict(scale=math.nan), dict(scale=0.0), dict(softcap=math.inf), dict(softcap=1e6), dict(softcap=-1.0),
+                                 dict(softcap=math.nan), dict(window=-1), dict(chunk=-1), dict(keep_first=-1), dict(window=4, chunk=4)], ids=str)
+def test_attention_options_that_have_no_answer(bad):
+    from mini_llama_cpp_release_b200.kernels import attention_quantised
+    c = PagedCache(needs()[:1], [None], [None], 640, 4, torch.float8_e4m3fn, torch.device("cpu"))
+    view = c.view(0, [torch.zeros(1, 1, dtype=torch.int32)])
+    q = torch.zeros(1, 2 * 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(KernelError, match="softcap"):
+        attention_quantised(q, q, i, i, 1, 1, 1, 2, view, **{**dict(scale=0.125), **bad})
+    with pytest.raises(KernelError, match="CUDA"):
+        attention_quantised(q, q, i, i, 1, 1, 1, 2, view, 0.125, softcap=2048.0)
+
+
+def test_what_a_soft_cap_rounds():
+    """cap * (1 - q), q = 2 / (1 + e^2y), in float32, the quotient two units off as a fast division may be, for scores of every size.  q <= 2: its two units are 2^-22 at most,
+    the exponential and the sum below it are rounded to 2^-24 of themselves and move q by 2^-23 each at most, the difference is rounded by 2^-24: together less than
+    cap * 2^-21.  So caps up to 2,048 stay within 2^-10, and one of a million would move a score by tenths."""
+    worst = {}
+    for cap in (0.5, 30.0, 2048.0, 1e6):
+        score = torch.linspace(-3.0, 3.0, 20001, dtype=torch.float64) * min(cap, 64.0) / 3.0
+        quotient = 2.0 / (1.0 + torch.exp(2.0 * score / cap).float())
+        for units in (-2, 0, 2):
+            got = cap * (1.0 - quotient * (1.0 + units * 2.0 ** -24)).double()
+            worst[cap] = max(worst.get(cap, 0.0), float((got - cap * torch.tanh(score / cap)).abs().max()))
+        assert worst[cap] < cap * 2.0 ** -21
+    assert worst[2048.0] <= 2.0 ** -10 and worst[1e6] > 0.1
