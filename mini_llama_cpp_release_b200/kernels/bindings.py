@@ -1356,7 +1356,7 @@ def check_gemm_status(device: torch.device) -> None:
                    61: "the float32 few-row product's wait for its operands", 71: "the 8-bit cache attention's loader",
                    72: "the 8-bit cache attention's wait for keys and values",
                    73: "the 8-bit cache prompt attention's loader", 74: "the 8-bit cache prompt attention's score issuer",
-                   75: "the 8-bit cache prompt attention's output issuer", 76: "the 8-bit cache prompt attention's rows or converters"}.get(code, str(code))
+                   75: "the 8-bit cache prompt attention's output issuer", 76: "the 8-bit cache prompt attention's rows"}.get(code, str(code))
             raise KernelError(f"a tcgen05 kernel gave up waiting on a barrier ({who}); its output is not valid")
 
 
