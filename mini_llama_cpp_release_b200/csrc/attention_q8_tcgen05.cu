@@ -319,8 +319,9 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         int done = 0;                             // tiles of this team
         for (int j = team; j < n_tiles; j += X_TEAMS, ++done) {
             const int i = j % X_AHEAD;
-            ok = mbar_wait(bar(XB_S_FULL + i), (unsigned)(j / X_AHEAD) & 1u, a.status, 76);
-            if (!ok) break;
+            // A thread whose wait ran out goes on with its warp, waits no more and stores nothing: tensor memory is read and written by whole warps.  (A vote on it in
+            // every tile instead: 405 to 414 us where this takes 397 to 405, as leaving the loop one by one did.)
+            if (ok) ok = mbar_wait(bar(XB_S_FULL + i), (unsigned)(j / X_AHEAD) & 1u, a.status, 76);
             tcgen05_fence_after();
             const unsigned s_addr = lanes + (unsigned)(i * X_KEYS);
             const int key0 = tile_of(j) * X_KEYS;
@@ -385,8 +386,7 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             l = l * corr + ((s0 + s1) + (s2 + s3));
             if (j >= X_TEAMS && __any_sync(0xffffffffu, raise)) {
                 // this warp's rows of the team's output, once the team's last product is complete
-                ok = mbar_wait(bar(XB_O_FULL + (j - X_TEAMS) % X_AHEAD), (unsigned)((j - X_TEAMS) / X_AHEAD) & 1u, a.status, 76);
-                if (!ok) break;
+                if (ok) ok = mbar_wait(bar(XB_O_FULL + (j - X_TEAMS) % X_AHEAD), (unsigned)((j - X_TEAMS) / X_AHEAD) & 1u, a.status, 76);
                 tcgen05_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < X_HD; c0 += 32) {

@@ -169,3 +169,21 @@ def test_what_a_soft_cap_rounds():
             worst[cap] = max(worst.get(cap, 0.0), float((got - cap * torch.tanh(score / cap)).abs().max()))
         assert worst[cap] < cap * 2.0 ** -21
     assert worst[2048.0] <= 2.0 ** -10 and worst[1e6] > 0.1
+
+
+def test_a_wait_that_ran_out_keeps_the_warp_together():
+    """What follows the row threads' waits (tensor memory, shuffles) is for whole warps.  So either the warp decides together whether a wait ran out, or the thread
+    stays: it waits no more (`if (ok) ok = ...`) and no loop over tiles is left by some lanes only."""
+    import os
+    import re
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    root = os.path.dirname(bindings._build.__file__)
+    for source, code in (("attention_q8_tcgen05.cu", "76"), ("attention_q8.cu", "72")):
+        with open(os.path.join(root, source)) as f:
+            lines = [re.sub(r"//.*", "", x).strip() for x in f]
+        waits = [i for i, x in enumerate(lines) if "mbar_wait(" in x and f"a.status, {code})" in x]
+        assert waits
+        for i in waits:
+            if "__all_sync(0xffffffffu, mbar_wait(" not in lines[i]:
+                assert lines[i].startswith("if (ok) ok = mbar_wait(") or lines[i - 1].startswith("if (ok && "), lines[i]
+                assert lines[i + 1] != "if (!ok) break;", lines[i]
