@@ -185,5 +185,5 @@ def test_a_wait_that_ran_out_keeps_the_warp_together():
         assert waits
         for i in waits:
             if "__all_sync(0xffffffffu, mbar_wait(" not in lines[i]:
-                assert lines[i].startswith("if (ok) ok = mbar_wait(") or lines[i - 1].startswith("if (ok && "), lines[i]
+                assert lines[i].startswith("if (ok) ok = mbar_wait(") or lines[i + 1] == "}", lines[i]
                 assert lines[i + 1] != "if (!ok) break;", lines[i]
