@@ -47,6 +47,27 @@ struct Q8Mask {
     __device__ __forceinline__ int kept() const { return window > 0 ? keep_first : 0; }
 };
 
+// Where the pages that a sequence's rows see lie among its expanded ones: tiles of kept first keys, then those from the first row's first key on.  What lies
+// between them nobody sees, and it has no place.
+struct Q8Places {
+    int head, gap;              // tiles of kept first keys before the gap, and its length
+    __device__ __forceinline__ Q8Places(const Q8Mask& mask, int start, int last_tile) {
+        const int first = min(mask.lowest(start) / 64, last_tile);
+        head = min(first, (mask.kept() + 63) / 64);
+        gap = first - head;
+    }
+    __device__ __forceinline__ int place(int tile) const { return tile < head ? tile : tile - gap; }
+    __device__ __forceinline__ int tile(int place) const { return place < head ? place : place + gap; }
+};
+// The most places that `tokens` new ones behind any number of keys need.
+static inline long long q8_places(long long tokens, int pages_per_seq, int window, int keep_first, int chunk) {
+    const long long pages = pages_per_seq > 1 ? pages_per_seq : 1;
+    if (window <= 0 && chunk <= 0) return pages;
+    const long long keys = (chunk > 0 ? chunk : window) + tokens - 1;                         // successive ones, from anywhere in a page on
+    const long long need = (keys + 62) / 64 + 1 + (window > 0 ? ((long long)keep_first + 63) / 64 : 0);
+    return need < pages ? need : pages;
+}
+
 struct Q8TcArgs {
     bf16* out;                  // [n_tokens][q_heads · hd]
     const int* cu_seqlens;
@@ -59,7 +80,7 @@ struct Q8TcArgs {
     int n_tokens;
     int q_heads, group, heads_per_block, tokens_per_block, head_chunks;
     Q8Mask mask;
-    int dense_tiles;            // tiles a sequence has in the expanded keys and values: [sequence][kv head][dense_tiles · 64][hd]
+    int dense_tiles;            // places a sequence has in the expanded keys and values: [sequence][kv head][dense_tiles · 64][hd]
     int row_tiles;              // of the longest sequence
     int whole_blocks;           // blocks before those that share a row tile's keys out
     int n_splits, split_tokens; // the first tokens of every sequence are split
@@ -72,24 +93,24 @@ struct Q8TcArgs {
 constexpr int X_HD = MLC_HEAD_DIM;
 constexpr int X_KEYS = 64;                             // keys of a tile: a page
 
-// ---------------- the expansion: a block a page of one kv head, keys and values; a lane eight numbers.  Only pages of tiles that some row of
-// the step sees; all 64 rows are written: values of rows that are not the sequence's, or whose page is missing, as zeros.
+// ---------------- the expansion: a block a place of one kv head, keys and values; a lane eight numbers.  Only pages of tiles that some row of
+// the step sees have one; all 64 rows are written: values of rows that are not the sequence's, or whose page is missing, as zeros.
 constexpr int XE_THREADS = 256;
 __global__ void __launch_bounds__(XE_THREADS) q8_expand_kernel(QuantisedKV c, const int* __restrict__ cu_seqlens, const int* __restrict__ start_pos, int n_tokens,
                                                                Q8Mask mask, int dense_tiles, bf16* __restrict__ k_dense, bf16* __restrict__ v_dense) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int b = blockIdx.z, kvh = blockIdx.y, tile = blockIdx.x;             // = page index
+    const int b = blockIdx.z, kvh = blockIdx.y, place = blockIdx.x;
     const int q_len = min(cu_seqlens[b + 1], n_tokens) - cu_seqlens[b];
     if (q_len <= 0) return;
-    const int start = start_pos[b], n_keys = start + q_len;
-    const int first = mask.lowest(start) / X_KEYS, head_tiles = (mask.kept() + X_KEYS - 1) / X_KEYS;
-    if (tile > (n_keys - 1) / X_KEYS || (tile < first && tile >= head_tiles)) return;
+    const int start = start_pos[b], n_keys = start + q_len, last_tile = max(c.pages_per_seq, 1) - 1;
+    const int tile = Q8Places(mask, start, last_tile).tile(place);
+    if (tile > min((n_keys - 1) / X_KEYS, last_tile)) return;
     const int page = tile < c.pages_per_seq ? __ldg(c.page_table + (long long)b * c.pages_per_seq + tile) : -1;
     const bool have = (unsigned)page < (unsigned)c.n_pages;
     const long long rows = ((long long)page * c.kv_heads + kvh) * X_KEYS;
     const int valid = have ? n_keys - tile * X_KEYS : 0;
-    const long long out_row = (((long long)b * c.kv_heads + kvh) * dense_tiles + tile) * X_KEYS;
+    const long long out_row = (((long long)b * c.kv_heads + kvh) * dense_tiles + place) * X_KEYS;
     constexpr int PER_ROW = X_HD / 8, STEPS = X_KEYS * PER_ROW / XE_THREADS;
     uint2 wk[STEPS], wv[STEPS];
     int bk[STEPS], bv[STEPS];
@@ -200,8 +221,9 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int p_first = start + tok0, p_last = p_first + n_tok - 1;
     const int keep = a.mask.kept();
     // tiles of kept first keys before the window's first tile are walked ahead of it; behind what a page list holds there are only missing pages
-    const int tile_begin = min(a.mask.lowest(p_first) / X_KEYS, a.dense_tiles - 1), head_tiles = min(tile_begin, (keep + X_KEYS - 1) / X_KEYS);
-    const int walk = n_tok > 0 ? head_tiles + min(p_last / X_KEYS, a.dense_tiles - 1) + 1 - tile_begin : 0;
+    const int last_tile = max(a.kv.pages_per_seq, 1) - 1;
+    const int tile_begin = min(a.mask.lowest(p_first) / X_KEYS, last_tile), head_tiles = min(tile_begin, (keep + X_KEYS - 1) / X_KEYS);
+    const int walk = n_tok > 0 ? head_tiles + min(p_last / X_KEYS, last_tile) + 1 - tile_begin : 0;
     const int j0 = parts ? (int)((long long)walk * split / a.n_splits) : 0;
     const int n_tiles = (parts ? (int)((long long)walk * (split + 1) / a.n_splits) : walk) - j0;
     const int heads_left = head_tiles - j0, shift = tile_begin - heads_left;               // (of this block's tiles)
@@ -222,6 +244,7 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             mbar_expect_tx(bar(XB_Q_FULL), (unsigned)(X_SPANS * a.heads_per_block * a.tokens_per_block * 128));
             for (int k = 0; k < X_SPANS; ++k) tma_load_3d(base + k * X_ROWS * 128, &map_q, k * 64, kvh * a.group + head0, seq_tok0 + tok0, bar(XB_Q_FULL));
             const int row0 = (b * a.kv.kv_heads + kvh) * a.dense_tiles;
+            const Q8Places places(a.mask, start, last_tile);
             // two streams, keys and values, each held up only by its own ring: the thread looks at both in turn
             int jk = 0, jv = 0;
             unsigned long long deadline = 0;
@@ -231,7 +254,7 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     const int s = jk % X_K_STAGES;
                     mbar_expect_tx(bar(XB_K_FULL + s), X_TILE_BYTES);
                     for (int k = 0; k < X_SPANS; ++k)
-                        tma_load_2d(base + X_K_OFF + s * X_TILE_BYTES + k * X_KEYS * 128, &map_k, k * 64, (row0 + tile_of(jk)) * X_KEYS, bar(XB_K_FULL + s));
+                        tma_load_2d(base + X_K_OFF + s * X_TILE_BYTES + k * X_KEYS * 128, &map_k, k * 64, (row0 + places.place(tile_of(jk))) * X_KEYS, bar(XB_K_FULL + s));
                     ++jk;
                     moved = true;
                 }
@@ -239,7 +262,7 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     const int s = jv % X_V_STAGES;
                     mbar_expect_tx(bar(XB_V_FULL + s), X_TILE_BYTES);
                     for (int k = 0; k < X_SPANS; ++k)
-                        tma_load_2d(base + X_V_OFF + s * X_TILE_BYTES + k * X_KEYS * 128, &map_v, k * 64, (row0 + tile_of(jv)) * X_KEYS, bar(XB_V_FULL + s));
+                        tma_load_2d(base + X_V_OFF + s * X_TILE_BYTES + k * X_KEYS * 128, &map_v, k * 64, (row0 + places.place(tile_of(jv))) * X_KEYS, bar(XB_V_FULL + s));
                     ++jv;
                     moved = true;
                 }
@@ -487,8 +510,7 @@ extern "C" int mlc_attention_q8_combine(const float* part_ml, const float* part_
 
 // As mlc_attention_q8, for head sizes of 64 and 128 (others are refused): 128 rows a block.  The keys of the last split_tiles row tiles to be
 // launched (every sequence's first ones) are shared out over n_splits blocks each; those need part_ml and part_o (layouts: Q8TcArgs, split_tokens = split_tiles ·
-// tokens of a block).  dense: scratch of
-// 2 · n_seqs · kv_heads · dense_tiles · 64 · head_dim bfloat16, with at least as many tiles as pages_per_seq (and one).
+// tokens of a block).  dense: scratch of 2 · n_seqs · kv_heads · dense_tiles · 64 · head_dim bfloat16, with at least the places of max_q_len tokens in whole blocks.
 extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_seqlens, const int* start_pos, int n_seqs, int n_tokens, int max_q_len,
                                         int q_heads, int kv_heads, int hd, float scale, int window, int keep_first, int chunk, float softcap,
                                         const float* sinks, int n_splits, int split_tiles, float* part_ml, float* part_o, void* dense, int dense_tiles,
@@ -504,7 +526,7 @@ extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)dense) & 15) return MLC_ERR_BAD_SIZE;
     if (entry_offset < 0 || entry_offset % ((long long)hd * X_KEYS) != 0) return MLC_ERR_BAD_SIZE;
     const long long dense_rows = (long long)n_seqs * kv_heads * dense_tiles * X_KEYS;
-    if (dense == nullptr || dense_tiles < 1 || dense_tiles < pages_per_seq || dense_rows > 0x7fffffffll || kv_heads > 65535 || n_seqs > 65535) return MLC_ERR_BAD_SIZE;
+    if (dense == nullptr || dense_tiles < 1 || dense_rows > 0x7fffffffll || kv_heads > 65535 || n_seqs > 65535) return MLC_ERR_BAD_SIZE;
     const long long scale_offset = entry_offset / hd;
     Q8TcArgs a{};
     a.out = (bf16*)out;
@@ -529,6 +551,7 @@ extern "C" int mlc_attention_q8_tcgen05(const void* q, void* out, const int* cu_
     a.cap_exponent = softcap > 0.0f ? 2.0f * 1.4426950408889634f * scale / softcap : 0.0f;
     a.row_tiles = (max_q_len + a.tokens_per_block - 1) / a.tokens_per_block;
     if (split_tiles > a.row_tiles) return MLC_ERR_BAD_SIZE;
+    if (dense_tiles < q8_places((long long)a.row_tiles * a.tokens_per_block, pages_per_seq, window, a.mask.keep_first, chunk)) return MLC_ERR_BAD_SIZE;
     const long long heads_seq = (long long)kv_heads * a.head_chunks * n_seqs, whole_blocks = heads_seq * (a.row_tiles - split_tiles);
     const long long blocks = whole_blocks + heads_seq * split_tiles * n_splits;
     if (blocks > 0x7fffffffll) return MLC_ERR_BAD_SIZE;

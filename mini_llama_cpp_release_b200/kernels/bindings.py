@@ -22,7 +22,7 @@ __all__ = [
     "group_norm", "activation", "forget_gate_attention", "moe_route_scored",
     "tanh_norm", "glu", "sigmoid_gate", "state_space",
     "decay_attention", "matrix_memory", "rms_pair", "embed_rms", "diff_combine", "moe_plan_table",
-    "QuantisedKVView", "quantise_kv", "dequantise_kv", "attention_quantised", "attention_q8_library", "attention_q8_plan", "attention_q8_tcgen05_plan",
+    "QuantisedKVView", "quantise_kv", "dequantise_kv", "attention_quantised", "attention_q8_library", "attention_q8_plan", "attention_q8_places", "attention_q8_tcgen05_plan",
 ]
 
 
@@ -1964,6 +1964,17 @@ def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
         return None
 
 
+def attention_q8_places(max_q_len: int, pages_per_seq: int, q_heads: int, kv_heads: int, window: int = 0, keep_first: int = 0, chunk: int = 0) -> int:
+    """Pages of a sequence that are written out as bfloat16 at most: those of its list, or under a mask those of kept first keys and of the keys that new tokens in whole
+    blocks of 128 rows see."""
+    pages = max(1, pages_per_seq)
+    if not (window or chunk):
+        return pages
+    tokens = 128 // min(q_heads // kv_heads, 128)
+    keys = (chunk or window) + -(-max_q_len // tokens) * tokens - 1            # successive ones, from anywhere in a page on
+    return min(pages, (keys + 62) // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
+
+
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
     """(n_splits, split_tiles) of the form with 128 rows a block, or None where it is not for these sizes: the keys of every sequence's first `split_tiles`
@@ -2036,7 +2047,7 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     dense = None
     if len(form) == 2:
         # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
-        dense_tiles = max(1, args[6])
+        dense_tiles = attention_q8_places(max_q_len, args[6], q_heads, kv.kv_heads, window, keep_first, chunk)
         dense = _spare_rows(n_seqs * kv.kv_heads * dense_tiles * 128 * kv.head_dim, q.device)
         if dense is None:
             form = attention_q8_plan(*sizes)

@@ -417,3 +417,21 @@ def test_rows_before_the_first_sequence_are_left_as_they_are(monkeypatch, form):
     assert (out[:before] == 7.0).all()
     c.q, c.cu = q, cu
     c.check(out[before:])
+
+
+@pytest.mark.parametrize("mask", [dict(window=100), dict(window=64, keep_first=65), dict(chunk=100)], ids=str)
+def test_pages_written_out_follow_the_mask_and_not_the_page_list(mask):
+    """A few new tokens far into long sequences whose layer has a mask: scratch for the pages that they see."""
+    c = Case(14, 2, 64, [(9000, 40), (30, 70), (6000, 1)], seed=51, tail=1)
+    out = torch.full_like(c.q, 7.0)
+    view = c.view()
+    c.run(out=out, **mask)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    kernels().attention_quantised(c.q, out, c.cu, c.start, 3, 70, 9040, 14, view, 0.125, **mask)
+    torch.cuda.synchronize()
+    # keys and values, 2 kv heads of 64 in bfloat16, at most 7 pages of each sequence (100 keys, 72 rows in whole blocks of 18 tokens, two kept pages)
+    assert kernels().attention_q8_tcgen05_plan(70, 3, 9040, 14, 2, 64, 148, **mask) == (1, 0)
+    assert torch.cuda.max_memory_allocated() - before <= 3 * 7 * 64 * 2 * 2 * 64 * 2 + 4096
+    c.check(out, **mask)

@@ -187,3 +187,28 @@ def test_a_wait_that_ran_out_keeps_the_warp_together():
             if "__all_sync(0xffffffffu, mbar_wait(" not in lines[i]:
                 assert lines[i].startswith("if (ok) ok = mbar_wait(") or lines[i + 1] == "}", lines[i]
                 assert lines[i + 1] != "if (!ok) break;", lines[i]
+
+
+def test_places_of_the_pages_that_are_written_out():
+    """Every page that some new token sees has a place of its own below the number that is asked for, wherever the sequence stands; under a mask that number follows the
+    mask and not the page list."""
+    import random
+    from mini_llama_cpp_release_b200.kernels import attention_q8_places
+    rng = random.Random(1)
+    for _ in range(4000):
+        kind = rng.choice(["all", "window", "kept", "chunk"])
+        size, keep = rng.randint(1, 700), rng.randint(1, 300) if kind == "kept" else 0
+        mask = {} if kind == "all" else dict(chunk=size) if kind == "chunk" else dict(window=size, keep_first=keep)
+        heads, kv_heads = rng.choice([(14, 2), (12, 2), (28, 4), (4, 4), (40, 2), (300, 1)])
+        block = 128 // min(heads // kv_heads, 128)
+        start, new = rng.randint(0, 4000), rng.randint(1, 300)
+        end = start + -(-new // block) * block                              # rows of the last block that do not exist take part in the walk
+        last = max(0, (start + new + 63) // 64 + rng.randint(-3, 40) - 1)   # of the page list, which may end before the sequence or go on behind it
+        lowest = 0 if kind == "all" else start // size * size if kind == "chunk" else max(0, start - size + 1)
+        n = attention_q8_places(rng.randint(new, end - start), last + 1, heads, kv_heads, **mask)
+        seen = [t for t in range(min((end - 1) // 64, last) + 1) if 64 * t + 63 >= lowest or t < -(-keep // 64)]
+        first = min(lowest // 64, last)                                     # the kernels' rule, csrc/attention_q8_tcgen05.cu (Q8Places)
+        head = min(first, -(-keep // 64))
+        places = [t if t < head else t - (first - head) for t in seen]
+        assert len(set(places)) == len(places) and all(0 <= x < n for x in places), (mask, start, new, last)
+        assert n <= last + 1 and (kind == "all" or n <= (size + end - start) // 64 + 2 + -(-keep // 64))
