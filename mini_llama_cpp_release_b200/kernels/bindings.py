@@ -1951,17 +1951,25 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
 # the half step to which the result is rounded.
 Q8_LARGEST_CAP = 2048.0
 Q8_CLUSTER = 8                  # the most key splits that join inside a thread-block cluster, without scratch memory and a second kernel
-EXPANDED_BYTES = 8 << 30        # the most scratch memory for pages written out as bfloat16 (a call that would want more runs in the form without)
+EXPANDED_BYTES = 8 << 30        # the most scratch memory for one sequence's pages written out as bfloat16 (beyond it a call runs in the form without)
+# And for several: a call takes as many at a time as it holds.  A captured step keeps its scratch while its graph is kept, so the limit is one that costs no time (504 MB in
+# all, 64 sequences of 16 new tokens behind 4,000, 28 heads of 128 on 4: 228 us at once, 229 in halves, 265 in quarters, 308 in eighths; 64 new: 503, 517, 480, 448).
+EXPANDED_AT_ONCE = 512 << 20
 
 
-def _spare_rows(n: int, device: torch.device) -> Optional[torch.Tensor]:
-    """n bfloat16 numbers of scratch memory; None where that is too much or there is no room for it."""
-    if 2 * n > EXPANDED_BYTES:
-        return None
-    try:
-        return torch.empty(n, dtype=torch.bfloat16, device=device)
-    except torch.OutOfMemoryError:
-        return None
+def _expanded_pages(per_seq: int, n_seqs: int, device: torch.device) -> Tuple[int, Optional[torch.Tensor]]:
+    """Scratch memory of `per_seq` bfloat16 numbers for as many sequences at a time as the limits and the free memory leave room for, in equal groups; (0, None) where not
+    even one has room."""
+    if 2 * per_seq > EXPANDED_BYTES:
+        return 0, None
+    at_once = min(n_seqs, max(1, EXPANDED_AT_ONCE // (2 * per_seq)))
+    while at_once:
+        at_once = -(-n_seqs // -(-n_seqs // at_once))
+        try:
+            return at_once, torch.empty(at_once * per_seq, dtype=torch.bfloat16, device=device)
+        except torch.OutOfMemoryError:
+            at_once //= 2
+    return 0, None
 
 
 def attention_q8_places(max_q_len: int, pages_per_seq: int, q_heads: int, kv_heads: int, window: int = 0, keep_first: int = 0, chunk: int = 0) -> int:
@@ -2044,34 +2052,38 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     sizes = (max_q_len, n_seqs, max_kv_len, q_heads, kv.kv_heads, kv.head_dim, _sm_counts.get(device) or _sm_count(q.device), window, keep_first, chunk)
     form = _attention_q8_form(*sizes)
     args = kv.args
-    dense = None
-    if len(form) == 2:
-        # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
-        dense_tiles = attention_q8_places(max_q_len, args[6], q_heads, kv.kv_heads, window, keep_first, chunk)
-        dense = _spare_rows(n_seqs * kv.kv_heads * dense_tiles * 128 * kv.head_dim, q.device)
-        if dense is None:
-            form = attention_q8_plan(*sizes)
-    part_tokens = n
-    if dense is not None:
-        (n_splits, split_tiles), in_cluster = form, False
-        part_tokens = n_seqs * split_tiles * (128 // min(q_heads // kv.kv_heads, 128))
-    else:
-        rows, n_splits, per_split, in_cluster = form
-    part_ml = part_o = None
-    joined_later = n_splits > 1 and not in_cluster
-    if joined_later:
-        part_ml = torch.empty(part_tokens * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
-        part_o = torch.empty(part_tokens * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
     status = _status.get(device)
     if status is None:
         status = gemm_status(q.device)
-    head = (q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, scale, window,
-            keep_first, chunk, softcap, _ptr(sinks))
-    if dense is not None:
-        rc = lib.mlc_attention_q8_tcgen05(*head, n_splits, split_tiles, _ptr(part_ml), _ptr(part_o), dense.data_ptr(), dense_tiles, *args, status.data_ptr(), _stream())
-        count_launches(1)
-    else:
-        rc = lib.mlc_attention_q8(*head, rows, n_splits, per_split, _ptr(part_ml), _ptr(part_o), *args, status.data_ptr(), _stream())
-    _check(rc, "attention over an 8-bit cache")
+    rest = (n, max_q_len, q_heads, kv.kv_heads, kv.head_dim, scale, window, keep_first, chunk, softcap, _ptr(sinks))
+    if len(form) == 2:
+        # (as many keys as a page list holds, not `max_kv_len`: a bound that is too small costs no keys)
+        dense_tiles = attention_q8_places(max_q_len, args[6], q_heads, kv.kv_heads, window, keep_first, chunk)
+        at_once, dense = _expanded_pages(kv.kv_heads * dense_tiles * 128 * kv.head_dim, n_seqs, q.device)
+        for first in range(0, n_seqs if at_once else 0, at_once or 1):
+            count = min(at_once, n_seqs - first)
+            n_splits, split_tiles = form if count == n_seqs else _attention_q8_form(max_q_len, count, *sizes[2:])
+            part_ml = part_o = None
+            if n_splits > 1:
+                part_rows = count * split_tiles * (128 // min(q_heads // kv.kv_heads, 128)) * q_heads * n_splits
+                part_ml = torch.empty(part_rows * 2, dtype=torch.float32, device=q.device)
+                part_o = torch.empty(part_rows * kv.head_dim, dtype=torch.float32, device=q.device)
+            # the group's bounds, starts and page lists; token numbers are the whole call's
+            _check(lib.mlc_attention_q8_tcgen05(q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr() + 4 * first, start_pos.data_ptr() + 4 * first, count, *rest,
+                                                n_splits, split_tiles, _ptr(part_ml), _ptr(part_o), dense.data_ptr(), dense_tiles, *args[:4],
+                                                args[4] + 4 * first * args[6], args[5] - first, *args[6:], status.data_ptr(), _stream()),
+                   "attention over an 8-bit cache")
+            count_launches(2 if n_splits > 1 else 1)
+        if at_once:
+            return
+        form = attention_q8_plan(*sizes)
+    rows, n_splits, per_split, in_cluster = form
+    part_ml = part_o = None
+    joined_later = n_splits > 1 and not in_cluster
+    if joined_later:
+        part_ml = torch.empty(n * q_heads * n_splits * 2, dtype=torch.float32, device=q.device)
+        part_o = torch.empty(n * q_heads * n_splits * kv.head_dim, dtype=torch.float32, device=q.device)
+    _check(lib.mlc_attention_q8(q.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(), start_pos.data_ptr(), n_seqs, *rest, rows, n_splits, per_split, _ptr(part_ml),
+                                _ptr(part_o), *args, status.data_ptr(), _stream()), "attention over an 8-bit cache")
     if joined_later:
         count_launches(1)

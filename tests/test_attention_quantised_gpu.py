@@ -435,3 +435,68 @@ def test_pages_written_out_follow_the_mask_and_not_the_page_list(mask):
     assert kernels().attention_q8_tcgen05_plan(70, 3, 9040, 14, 2, 64, 148, **mask) == (1, 0)
     assert torch.cuda.max_memory_allocated() - before <= 3 * 7 * 64 * 2 * 2 * 64 * 2 + 4096
     c.check(out, **mask)
+
+
+class Spy:
+    """A library of attention kernels that notes which entry point a call went through."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        f = getattr(self.lib, name)
+        return lambda *a: (self.calls.append(name), f(*a))[1]
+
+
+def spied(monkeypatch, hd):
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    spy = Spy(kernels().attention_q8_library(hd))
+    monkeypatch.setitem(bindings._attn_q8_libs, hd, spy)
+    return spy
+
+
+GROUPS = [(70, 90), (0, 150), (500, 3), (10, 0), (700, 20), (64, 64), (0, 1)]
+
+
+@pytest.mark.parametrize("at_once", [1, 2, 3, 6])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("mask", [dict(), dict(sinks=True, softcap=5.0), dict(window=70, keep_first=65, sinks=True), dict(chunk=100)],
+                         ids=["all", "sinks", "window", "chunk"])
+def test_as_many_sequences_at_a_time_as_scratch_memory_holds(monkeypatch, H, KV, hd, mask, at_once):
+    """The sequences' pages are written out in groups: every sequence as in one call for all, one without new tokens, a missing page and rows behind the last among them."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    spy = spied(monkeypatch, hd)
+    c = Case(H, KV, hd, GROUPS, seed=52, tail=3)
+    places = kernels().attention_q8_places(150, c.table.shape[1], H, KV, mask.get("window", 0), mask.get("keep_first", 0), mask.get("chunk", 0))
+    per_seq = KV * places * 64 * hd * 2 * 2
+    monkeypatch.setattr(bindings, "EXPANDED_AT_ONCE", at_once * per_seq + per_seq // 2)
+    monkeypatch.setattr(bindings, "EXPANDED_BYTES", per_seq)
+    c.check(c.run(**mask), **mask)
+    assert spy.calls == ["mlc_attention_q8_tcgen05"] * -(-len(GROUPS) // at_once)
+    table = c.table.clone()
+    table[0, 0] = table[4, 3] = -1
+    c.check(c.run(table=table, **mask), gone=[(0, 0), (4, 3)], **mask)
+
+
+def test_scratch_memory_that_is_short_halves_the_groups(monkeypatch):
+    """Where several sequences' pages find no room, fewer at a time are tried, down to one, before the form without is taken."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    spy = spied(monkeypatch, 64)
+    c = Case(14, 2, 64, GROUPS, seed=53, tail=1)
+    per_seq = 2 * c.table.shape[1] * 128 * 64
+    empty = torch.empty
+
+    def short(n, *a, **k):
+        if k.get("dtype") == torch.bfloat16 and n > room:
+            raise torch.OutOfMemoryError("no room")
+        return empty(n, *a, **k)
+
+    monkeypatch.setattr(bindings.torch, "empty", short)
+    for room, calls in ((3 * per_seq, 3), (per_seq, 7)):
+        del spy.calls[:]
+        c.check(c.run(out=torch.full_like(c.q, 7.0)))
+        assert spy.calls == ["mlc_attention_q8_tcgen05"] * calls
+    room = per_seq - 1
+    del spy.calls[:]
+    c.check(c.run(out=torch.full_like(c.q, 7.0)))
+    assert spy.calls == ["mlc_attention_q8"]

@@ -212,3 +212,23 @@ def test_places_of_the_pages_that_are_written_out():
         places = [t if t < head else t - (first - head) for t in seen]
         assert len(set(places)) == len(places) and all(0 <= x < n for x in places), (mask, start, new, last)
         assert n <= last + 1 and (kind == "all" or n <= (size + end - start) // 64 + 2 + -(-keep // 64))
+
+
+def test_scratch_memory_for_pages_written_out(monkeypatch):
+    """Several sequences take half a GiB at most, one as much as it needs up to the limit, in equal groups; fewer at a time where there is no room."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    made = []
+
+    def empty(n, dtype, device):
+        if 2 * n > room:
+            raise torch.OutOfMemoryError("no room")
+        made.append(n)
+        return n
+
+    monkeypatch.setattr(bindings.torch, "empty", empty)
+    for per_seq, n_seqs, room, want in ((1000, 7, 1 << 40, 7), (1 << 26, 128, 1 << 40, 4), (1 << 26, 9, 1 << 40, 3), (1 << 26, 5, 1 << 40, 3), (1 << 30, 3, 1 << 40, 1), (1 << 32, 1, 1 << 40, 1),
+                                        ((1 << 32) + 1, 1, 1 << 40, 0), (1 << 26, 128, 1 << 28, 2), (1 << 26, 128, 1 << 27, 1), (1 << 26, 128, (1 << 27) - 1, 0)):
+        del made[:]
+        at_once, tensor = bindings._expanded_pages(per_seq, n_seqs, torch.device("cpu"))
+        assert at_once == want and (tensor == want * per_seq if want else tensor is None) and len(made) == bool(want), (per_seq, n_seqs, room)
+        assert want <= 1 or 2 * want * per_seq <= bindings.EXPANDED_AT_ONCE
