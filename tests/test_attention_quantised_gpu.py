@@ -500,3 +500,103 @@ def test_scratch_memory_that_is_short_halves_the_groups(monkeypatch):
     del spy.calls[:]
     c.check(c.run(out=torch.full_like(c.q, 7.0)))
     assert spy.calls == ["mlc_attention_q8"]
+
+
+@pytest.fixture(params=[(14, 2, 64), (12, 2, 128), (28, 4, 128), (5, 1, 64)], ids=str)
+def without_scratch(request, monkeypatch):
+    """Layouts whose many-token calls run in the form without scratch pages, 64 rows a block, because there is no room for them; that they do is checked."""
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    monkeypatch.setattr(bindings, "EXPANDED_BYTES", 0)
+    spy = spied(monkeypatch, request.param[2])
+    yield request.param
+    assert spy.calls and set(spy.calls) == {"mlc_attention_q8"}
+
+
+@pytest.mark.parametrize("seqs", CHUNKS[1:], ids=[str(i) for i in range(1, len(CHUNKS))])
+def test_chunks_without_scratch(without_scratch, seqs):
+    c = Case(*without_scratch, seqs, seed=60, tail=3)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("mask", MASKS, ids=[str(m) for m in MASKS])
+def test_chunks_with_masks_without_scratch(without_scratch, mask):
+    c = Case(*without_scratch, [(700, 150), (0, 1), (0, 260), (100, 5), (1500, 40)], seed=61)
+    c.check(c.run(**mask), **mask)
+
+
+@pytest.mark.parametrize("mask", [dict(), dict(window=100, keep_first=4, sinks=True)], ids=["all", "window"])
+def test_missing_pages_without_scratch(without_scratch, mask):
+    c = Case(*without_scratch, [(300, 200), (0, 70), (30, 100)], seed=62)
+    table = c.table.clone()
+    table[0, 2], table[1, 0], table[2, :] = -1, 10 ** 6, -1
+    out = c.run(table=table, **mask)
+    c.check(out, gone=[(0, 2), (1, 0)] + [(2, p) for p in range(table.shape[1])], **mask)
+    assert not out[270:].any()
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["keys", "values"])
+@pytest.mark.parametrize("softcap", [0.0, 4.0])
+def test_a_row_that_is_not_finite_without_scratch(without_scratch, which, softcap):
+    H, KV, hd = without_scratch
+    c = Case(H, KV, hd, [(130, 100), (130, 100)], seed=63)
+    clean = c.run(window=50, softcap=softcap).view(-1, H, hd)
+    c.check(clean.view(c.n, -1), window=50, softcap=softcap)
+    c.codes[which][1, c.table[0, 2], KV - 1, 12] = 0                # key 140 of sequence 0
+    c.scales[which][1, c.table[0, 2], KV - 1, 12] = 255
+    out = c.run(window=50, softcap=softcap).view(-1, H, hd)
+    p = torch.arange(130, 230, device="cuda")
+    hit = torch.zeros(out.shape[0], H, dtype=torch.bool, device="cuda")
+    hit[:100, H - H // KV:] = ((140 <= p) & (p - 140 < 50))[:, None]
+    assert torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("softcap,size", [(0.5, 40.0), (30.0, 60.0), (50.0, 0.01)])
+def test_capped_scores_without_scratch(without_scratch, softcap, size):
+    c = Case(*without_scratch, [(70, 90), (0, 129)], seed=64, q_size=size)
+    c.check(c.run(softcap=softcap), softcap=softcap)
+
+
+def test_long_chunks_in_two_shares_without_scratch(without_scratch):
+    c = Case(*without_scratch, [(6000, 300), (6100, 90)], seed=65, tail=1)
+    c.check(c.run())
+
+
+SHORT = [(14, 2, 64), (12, 2, 128), (28, 4, 128), (48, 8, 64), (10, 2, 128)]
+
+
+@pytest.mark.parametrize("H,KV,hd", SHORT)
+@pytest.mark.parametrize("new", range(2, 11))
+def test_short_turns_behind_hundreds_of_keys(H, KV, hd, new):
+    """2 to 10 new tokens with groups of 5 to 7: every form by number of rows, and ragged beside single tokens."""
+    c = Case(H, KV, hd, [(700, new), (333, 1), (64 * 5 - new, new), (0, new), (450, max(1, new - 3))], seed=66, tail=2)
+    c.check(c.run())
+    c.check(c.run(window=130, keep_first=3, sinks=True, softcap=20.0), window=130, keep_first=3, sinks=True, softcap=20.0)
+
+
+@pytest.mark.parametrize("H,hd", [(28, 128), (12, 128), (20, 64), (28, 48)])
+@pytest.mark.parametrize("seqs", [[(500, 1), (20, 1), (3000, 1)], [(700, 2), (90, 2)], [(300, 200), (0, 33), (64, 1)]], ids=["single", "two", "chunk"])
+def test_shared_rows_for_many_heads(H, hd, seqs):
+    """One row of keys that are the values too, for up to 28 heads: more than a block of single tokens takes."""
+    c = Case(H, 1, hd, seqs, seed=67, shared=True, tail=1)
+    c.check(c.run())
+    c.check(c.run(window=100, keep_first=2, sinks=True), window=100, keep_first=2, sinks=True)
+
+
+@pytest.mark.parametrize("group", range(1, 17))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_every_group_of_single_tokens_joined_in_clusters(hd, group):
+    """Rows that fill a warp's columns and rows that do not, in a cluster of blocks that join among themselves."""
+    plan = kernels().attention_q8_plan(1, 2, 2001, group, 1, hd, torch.cuda.get_device_properties(0).multi_processor_count)
+    assert plan[1] > 1 and plan[3]
+    c = Case(group, 1, hd, [(2000, 1), (77, 1)], seed=68, tail=1)
+    c.check(c.run())
+    c.check(c.run(sinks=True, softcap=8.0), sinks=True, softcap=8.0)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (28, 1, 128)])
+@pytest.mark.parametrize("seqs", [[(2000, 1)], [(8000, 1), (17, 1)], [(20000, 1)] * 2, [(3000, 1)] * 90, [(700, 6)] * 3, [(900, 150)], [(30, 90), (500, 40)]], ids=str)
+def test_every_form_gives_the_same_bits_again(H, KV, hd, seqs):
+    c = Case(H, KV, hd, seqs, seed=69)
+    first = c.run()
+    for _ in range(3):
+        assert torch.equal(first, c.run())

@@ -218,3 +218,61 @@ def test_no_row_of_the_cache_is_written_twice_in_a_step(n, monkeypatch):
             places = [(int(table[s, p // 64]), int(p) % 64) for p, s in zip(positions.tolist(), tok_seq.tolist()) if s >= 0]
             assert len(set(places)) == len(places)
     assert any(t.shape[0] > n - 1 for _, t, _ in calls[2:])
+
+
+@pytest.mark.parametrize("name", ["C", "D", "kebesun/attention", "lonulix/latent"])
+def test_prompt_steps_replayed_from_their_graph(name):
+    """A step whose shape comes again is captured and replayed: other tokens in other slots, and a second chunk of each, give what the same steps give issued one by one,
+    and the first layer's cached rows follow from the tokens."""
+    f = folder(name)
+    vocab = ml.ModelConfig.from_folder(f).vocab_size
+    steps = [[helpers.random_tokens(n, vocab, 100 * k + n) for n in (90, 71, 90)] for k in range(4)]
+    more = [[helpers.random_tokens(n, vocab, 50 + 100 * k + n) for n in (70, 70, 66)] for k in range(4)]
+    kept = []
+    for graphs in (True, False):
+        ctx = ml.load(f, max_tokens=4096, cache_dtype="float8_e4m3").context
+        ctx.use_graphs = graphs
+        out = []
+        for first, second in zip(steps, more):
+            slots = [ctx.acquire() for _ in first]
+            logits = [ctx.forward_batch(MiniBatch.prefill(slots, x)).float().cpu().clone() for x in (first, second)]
+            entry = next(e for e, w in enumerate(ctx.cache.where) if w is not None)
+            out.append((logits, [ctx.cache.read(entry, s) for s in slots]))
+        assert len(getattr(ctx, "_step_graphs", {})) == (2 if graphs else 0)
+        kept.append(out)
+    for (logits, rows), (other, other_rows) in zip(*kept):
+        for a, b in zip(logits, other):
+            assert (a - b).abs().max() <= helpers.TOL["bfloat16"] * b.abs().max()
+        for pair, other_pair in zip(rows, other_rows):
+            for x, y in zip(pair, other_pair):
+                assert (x is None) == (y is None) and (x is None or torch.equal(x, y))
+
+
+def test_a_step_with_spare_rows_writes_none_of_them(monkeypatch):
+    """Batches that a captured step has more rows for than sequences: the step's rows past the sequences are marked, at every step and after the batch has changed."""
+    import mini_llama_cpp_release_b200.kernels as kernels
+    calls = []
+    quantise = kernels.quantise_kv
+
+    def spy(k, v, positions, tok_seq, kv):
+        calls.append(tok_seq)
+        quantise(k, v, positions, tok_seq, kv)
+
+    monkeypatch.setattr(kernels, "quantise_kv", spy)
+    ctx = ml.load(folder("C"), max_tokens=4096, cache_dtype="float8_e4m3").context
+    slots = [ctx.acquire() for _ in range(16)]
+    ctx.forward_batch(MiniBatch.prefill(slots, [helpers.random_tokens(10 + i, 777, 90 + i) for i in range(16)]))
+    sampler = DeviceSampler(SamplingParams(), ctx.model.runtime.device)
+    spare = 0
+    for live in (16, 13, 15, 11, 9, 5, 7, 3, 6):
+        before = len(calls)
+        for _ in range(2):
+            ctx.decode_and_sample(slots[:live], list(range(live)), sampler, list(range(live)))
+        torch.cuda.synchronize()
+        runner = next(reversed(ctx._runners.values()))
+        assert len(calls) > before or runner.n_live == live                # captured now, or a captured step that was loaded again
+        seq = runner.view("store_seq")
+        assert any(t.data_ptr() == seq.data_ptr() for t in calls)
+        assert seq.tolist() == list(range(live)) + [-1] * (runner.B - live)
+        spare += runner.B > live
+    assert spare >= 4
