@@ -95,7 +95,6 @@ class DecodeRunner:
         self.dev_buf = torch.zeros(total, dtype=torch.int32, device=dev)
         self.host_buf = torch.zeros(total, dtype=torch.int32).pin_memory()
         self.host_np = self.host_buf.numpy()                       # the same pinned memory, for cheap writes from lists
-        self.step_inputs = 4 * B                                    # ints copied to the device at every step
         self.history = torch.zeros(self.HISTORY_STEPS, B, dtype=torch.int32, device=dev)
         self.chosen_host = torch.zeros(B, dtype=torch.int32).pin_memory()
         self.slots_long = torch.zeros(B, dtype=torch.int64, device=dev)
