@@ -91,11 +91,17 @@ def _row_bytes(need: CacheNeed, itemsize: int, scales: int = 0) -> int:
     return (1 if need.shared_kv else 2) * need.kv_heads * (need.head_dim * itemsize + scales)
 
 
-def cache_bytes_per_token(needs: Sequence[Optional[CacheNeed]], reads_cache_of: Sequence[Optional[int]], itemsize: int) -> int:
-    """Key and value bytes one token of one sequence occupies over all groups, for elements of `itemsize` bytes
+def cache_bytes_per_token(needs: Sequence[Optional[CacheNeed]], reads_cache_of: Sequence[Optional[int]], itemsize: int, scales: int = 0) -> int:
+    """Key and value bytes one token of one sequence occupies over all groups, for elements of `itemsize` bytes and `scales` bytes a row
     (a window group holds at most its window of them)."""
     groups, _ = plan_groups(needs, reads_cache_of)
-    return sum(len(g.entries) * _row_bytes(g.need, itemsize) for g in groups)
+    return sum(len(g.entries) * _row_bytes(g.need, itemsize, scales) for g in groups)
+
+
+def takes_eight_bits(mixer) -> bool:
+    """Whether an 8-bit cache can hold what this mixer caches (True of one that caches nothing)."""
+    need = mixer.cache_need() if hasattr(mixer, "cache_need") else None
+    return need is None or (getattr(mixer, "takes_quantised_cache", False) and need.head_dim % 16 == 0 and need.head_dim <= 256)
 
 
 class SlotBook:

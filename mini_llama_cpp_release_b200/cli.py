@@ -246,7 +246,7 @@ def cmd_inspect(argv: Sequence[str]) -> int:
     model, config_path = resolve_model(args)
     from mini_llama_cpp_release_b200.config import ModelConfig, build_model_spec
     from mini_llama_cpp_release_b200.engine.model import build_parts
-    from mini_llama_cpp_release_b200.cache.paged import cache_bytes_per_token
+    from mini_llama_cpp_release_b200.cache.paged import cache_bytes_per_token, takes_eight_bits
     from mini_llama_cpp_release_b200.weights import Checkpoint, compare, expected_tensors
     from mini_llama_cpp_release_b200.weights.loader import ignorable_tensors
     cfg = ModelConfig.from_folder(config_path or (model if os.path.isdir(model) else os.path.join(os.path.dirname(model) or ".", "config.json")))
@@ -271,8 +271,10 @@ def cmd_inspect(argv: Sequence[str]) -> int:
     # what the runs of the schedule declare that they keep, asked of the cache's own planner
     mixers = [getattr(parts.blocks[e.layer], "mixer", None) for e in spec.schedule]
     needs = [m.cache_need() if hasattr(m, "cache_need") else None for m in mixers]
-    kv = cache_bytes_per_token(needs, [e.reads_cache_of for e in spec.schedule], 1)
-    print(f"cache per token per sequence: {kv * 2} B in bfloat16, {kv * 4} B in float32")
+    reads = [e.reads_cache_of for e in spec.schedule]
+    kv = cache_bytes_per_token(needs, reads, 1)
+    eight = f"{cache_bytes_per_token(needs, reads, 1, 1)} B in float8_e4m3" if all(map(takes_eight_bits, mixers)) else "not in 8 bits"
+    print(f"cache per token per sequence: {kv * 2} B in bfloat16, {kv * 4} B in float32, {eight}")
     # fixed-size state of the mixers that keep one (recurrences, convolutions), whatever the sequence's length
     import math
     import torch

@@ -232,3 +232,11 @@ def test_scratch_memory_for_pages_written_out(monkeypatch):
         at_once, tensor = bindings._expanded_pages(per_seq, n_seqs, torch.device("cpu"))
         assert at_once == want and (tensor == want * per_seq if want else tensor is None) and len(made) == bool(want), (per_seq, n_seqs, room)
         assert want <= 1 or 2 * want * per_seq <= bindings.EXPANDED_AT_ONCE
+
+
+@pytest.mark.parametrize("name,want", [("A", "256 B in bfloat16, 512 B in float32, 136 B in float8_e4m3"), ("kebesun/big_latent", "not in 8 bits")])
+def test_inspect_says_what_a_token_takes_in_8_bits(name, want, capsys):
+    import helpers
+    folder = helpers.model_folder(name) if "/" not in name else __import__(name.split("/")[0] + "_helpers").folder_of(name.split("/")[1])
+    assert cli.main(["inspect", folder]) == 0
+    assert want in capsys.readouterr().out
