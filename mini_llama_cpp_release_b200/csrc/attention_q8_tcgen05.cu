@@ -4,7 +4,7 @@
 // The scales are powers of two, so a row's numbers are bfloat16 numbers exactly.  q8_expand_kernel writes the pages that the step's rows
 // see as dense bfloat16 rows once, and the products are those of a bfloat16 cache.  The other places for that conversion were measured and
 // cost more: codes turned into tiles in shared memory by four or eight warps of the attention block itself, anew for every 256 rows
-// (B200, whole calls, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so when the two were compared, 11 of them the expansion; 404 now;
+// (B200, whole calls, 2,048 tokens behind 14,000, 28 heads of 128 on 4: 590 us, and 480 so when the two were compared, 11 of them the expansion; 383 to 412 now;
 // 4,095 tokens, 14 heads of 64 on 2: 67, and 55, 6 of them: the conversions' instructions and shared-memory traffic hold up the rows and the products alike).
 //
 // A block owns 128 rows of one kv head (the group's query heads of 128 / group successive tokens; a row is a token and a head) and walks the
@@ -15,6 +15,9 @@
 //     warps 3-     teams of four warps, a thread a row: three teams with a head size of 64, two with 128; team t takes the tiles t, t + teams, ...  Mask,
 //                  running maximum and sum in float32, probabilities as bfloat16 back into tensor memory over the scores.  A team has an output of its own in
 //                  tensor memory, rescaled only when a row's maximum rises by 2^8; at the end the teams' outputs are added.
+// The probabilities have the values' type because one product takes one: bfloat16 holds every row of the cache, float16 would not, and tf32 has
+// half the rate.  That rounding, 2^-8 a probability, is what the result has beside its own: relative error (of the norm) 0.0017 to 0.0020 where
+// a result that is only rounded at the end has 0.0015 to 0.0017.
 // What bounds a tile of 128 x 64: 512 clocks of exponentials, 320 (head size 64) or 640 (128) of products; it takes some 640 and 880, since a row's
 // chain of a tile (scores, maximum, exponentials, probabilities handed over) is 1,900 clocks long and only the teams overlap.  Blocks of 256 rows, a team a
 // row tile, with tiles of 128 keys took 562 and 63 us a call where these took 500 and 55 on that GPU.
@@ -342,8 +345,9 @@ attention_q8_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         int done = 0;                             // tiles of this team
         for (int j = team; j < n_tiles; j += X_TEAMS, ++done) {
             const int i = j % X_AHEAD;
-            // A thread whose wait ran out goes on with its warp, waits no more and stores nothing: tensor memory is read and written by whole warps.  (A vote on it in
-            // every tile instead: 405 to 414 us where this takes 397 to 405, as leaving the loop one by one did.)
+            // A thread whose wait ran out goes on with its warp, waits no more and stores nothing: tensor memory is read and written by whole warps.  (2,048 tokens behind
+            // 14,000, whole calls in turn on one GPU: 425 us; with a vote on it in every tile 427, with the mask's vote for both 432, with lanes that left the loop one by one,
+            // which is not sound, 419.)
             if (ok) ok = mbar_wait(bar(XB_S_FULL + i), (unsigned)(j / X_AHEAD) & 1u, a.status, 76);
             tcgen05_fence_after();
             const unsigned s_addr = lanes + (unsigned)(i * X_KEYS);

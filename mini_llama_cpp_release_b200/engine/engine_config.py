@@ -52,7 +52,9 @@ class EngineConfig:
                          cuts a larger batch into several steps, sequence by sequence;
     cache_dtype          what cached keys and values are held in: None for `dtype`, or "float8_e4m3" (bfloat16 engines): one byte
                          a number and one a row of a head, half the memory and half the bytes a decoded token reads, keys and values
-                         rounded to four significant bits."""
+                         rounded to four significant bits.  Steps of several tokens a sequence write one layer's visible pages out in 16
+                         bits: scratch memory beside the cache, four bytes a number, up to half a GiB for the sequences that run
+                         together (more for a single one that needs it), which a captured step keeps while its graph is kept."""
     dtype: object = "bfloat16"
     device: str = "cuda:0"
     max_tokens: int = 8192

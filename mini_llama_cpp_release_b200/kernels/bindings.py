@@ -1986,7 +1986,12 @@ def attention_q8_places(max_q_len: int, pages_per_seq: int, q_heads: int, kv_hea
 def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int, n_sms: int, window: int = 0,
                               keep_first: int = 0, chunk: int = 0):
     """(n_splits, split_tiles) of the form with 128 rows a block, or None where it is not for these sizes: the keys of every sequence's first `split_tiles`
-    row tiles are shared out over n_splits blocks."""
+    row tiles are shared out over n_splits blocks.
+
+    From 64 rows of a kv head on this form is the sooner one, whatever else the call holds, though it writes out pages that a short turn reads once, and gives a single token beside
+    a longer turn a block of 128 rows.  us on B200, this form and the one without scratch pages, 28 heads of 128 on 4: 16 new tokens behind 500, 12 and 16; 4 sequences of 16 behind
+    4,000, 26 and 68; 16 of 16 behind 8,000, 125 and 250 (its bytes: 21); 64 of 16 behind 4,000, 227 and 475; 63 single tokens at 4,000 beside one prompt of 16, 220 and 242,
+    of 512, 301 and 472; at 1,000 beside 16, 63 and 66.  Of 231 such shapes one went the other way: 63 single tokens at 1,000 beside a prompt of 2,048, 14 heads of 64 on 2, 201 and 161."""
     group = q_heads // kv_heads
     if head_dim not in TCGEN05_ATTENTION_HEAD_DIMS or max_q_len < 2 or max_q_len * group < 64:
         return None
@@ -1999,7 +2004,7 @@ def attention_q8_tcgen05_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_he
         longest = min(longest, ((chunk or window) + tokens + 126) // 64 + 1 + ((keep_first + 63) // 64 if window else 0))
     # Blocks run in whole waves, and what is left over would take as long as a full one: its keys are shared out where that is sooner.  In tiles: a block's start and
     # end are eight, the joining twelve, 0.3 a block's rows and 0.1 their share of a split (512 new behind 20,000, 28 heads of 128 on 4, 116 blocks: 156 us, in two
-    # splits 186; 2,048 behind 14,000, 456 blocks, 12 of them in twelve splits each: 404 us, 451 without; behind 30,000: 811 and 927; 100 behind 30,000, 14 heads of 64 on 2,
+    # splits 186; 2,048 behind 14,000, 456 blocks, 12 of them in twelve splits each: 383 to 412 us, 451 without; behind 30,000: 811 and 927; 100 behind 30,000, 14 heads of 64 on 2,
     # 12 blocks: 31 and 172).  Behind full waves only for one sequence: the lengths of several are not known here.
     split_tiles = row_tiles - row_tiles * across // n_sms * n_sms // across
     left = split_tiles * across
