@@ -600,3 +600,14 @@ def test_every_form_gives_the_same_bits_again(H, KV, hd, seqs):
     first = c.run()
     for _ in range(3):
         assert torch.equal(first, c.run())
+
+
+@pytest.mark.parametrize("width", [0, 1, 3, 9])
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (12, 2, 128), (6, 2, 48)])
+@pytest.mark.parametrize("seqs", [[(700, 1), (64, 1), (20, 1)], [(700, 150), (0, 260), (100, 5), (560, 40)]], ids=["single", "chunk"])
+@pytest.mark.parametrize("mask", [dict(), dict(window=100), dict(window=64, keep_first=130, sinks=True), dict(chunk=100, softcap=5.0)], ids=str)
+def test_page_lists_that_end_before_the_sequences(H, KV, hd, seqs, mask, width):
+    """Keys behind what a list holds are not seen, and a list may hold nothing."""
+    c = Case(H, KV, hd, seqs, seed=70, tail=1)
+    table = c.table[:, :width].contiguous()
+    c.check(c.run(table=table, **mask), gone=[(b, p) for b in range(len(seqs)) for p in range(width, c.table.shape[1])], **mask)
