@@ -1946,6 +1946,12 @@ def attention_q8_plan(max_q_len: int, n_seqs: int, max_kv_len: int, q_heads: int
     return rows, -(-tiles // run), run, False
 
 
+def _q8_mask(window: int, keep_first: int, chunk: int) -> Tuple[int, int, int]:
+    """A mask's lengths as the kernels take them, in 32 bits with room for a page above: no position is as far as the largest of them, so a longer one masks the same."""
+    return min(window, Q8_LONGEST), min(keep_first, Q8_LONGEST), min(chunk, Q8_LONGEST)
+
+
+Q8_LONGEST = (1 << 31) - 256
 # The largest soft cap c.  The kernels compute c · (1 - 2 / (1 + e^2y)) in float32.  The quotient q is 2 at most; two units of a fast division are 2^-22, the exponential's
 # and the sum's roundings 2^-24 of q each, the difference's 2^-24: a score is off by less than c · 2^-21.  At 2,048 that is 2^-10, and what it moves a weight by comes up to
 # the half step to which the result is rounded.
@@ -2035,6 +2041,7 @@ def attention_quantised(q: torch.Tensor, out: torch.Tensor, cu_seqlens: torch.Te
     if not 0 < scale < float("inf") or window < 0 or keep_first < 0 or chunk < 0 or not 0 <= softcap <= Q8_LARGEST_CAP or (window and chunk):
         raise KernelError(f"attention over an 8-bit cache: scale {scale}, window {window}, keep_first {keep_first}, chunk {chunk}, softcap {softcap} "
                           f"(at most {Q8_LARGEST_CAP})")
+    window, keep_first, chunk = _q8_mask(window, keep_first, chunk)
     device = kv.check()
     _on_device(device, q, out, cu_seqlens, start_pos, sinks)
     n = q.shape[0]

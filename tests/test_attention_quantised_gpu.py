@@ -611,3 +611,13 @@ def test_page_lists_that_end_before_the_sequences(H, KV, hd, seqs, mask, width):
     c = Case(H, KV, hd, seqs, seed=70, tail=1)
     table = c.table[:, :width].contiguous()
     c.check(c.run(table=table, **mask), gone=[(b, p) for b in range(len(seqs)) for p in range(width, c.table.shape[1])], **mask)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(14, 2, 64), (6, 2, 48)])
+@pytest.mark.parametrize("seqs", [[(700, 1), (64, 1)], [(700, 90), (0, 130)]], ids=["single", "chunk"])
+@pytest.mark.parametrize("mask,same", [(dict(window=(1 << 32) + 5), dict()), (dict(chunk=1 << 40), dict()), (dict(window=3, keep_first=(1 << 31) - 1), dict()),
+                                       (dict(window=(1 << 31) - 1, keep_first=4), dict())], ids=str)
+def test_masks_longer_than_any_sequence(H, KV, hd, seqs, mask, same):
+    c = Case(H, KV, hd, seqs, seed=71, tail=1)
+    out = c.run(**mask)
+    c.check(out, **same)

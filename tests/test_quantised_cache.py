@@ -240,3 +240,29 @@ def test_inspect_says_what_a_token_takes_in_8_bits(name, want, capsys):
     folder = helpers.model_folder(name) if "/" not in name else __import__(name.split("/")[0] + "_helpers").folder_of(name.split("/")[1])
     assert cli.main(["inspect", folder]) == 0
     assert want in capsys.readouterr().out
+
+
+def test_lengths_of_masks_past_32_bits(monkeypatch):
+    """A window, kept keys or a chunk longer than any sequence reaches the kernels as the longest length that 32 bits hold with a page above it, not as its low bits."""
+    import types
+    import mini_llama_cpp_release_b200.kernels.bindings as bindings
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: seen.append((name, a)) or 0
+
+    for patch in (("_on_device", lambda *a: None), ("_sm_count", lambda d: 148), ("_stream", lambda: 0), ("gemm_status", lambda d: torch.zeros(1, dtype=torch.int32))):
+        monkeypatch.setattr(bindings, *patch)
+    monkeypatch.setitem(bindings._attn_q8_libs, 64, Lib())
+    kv = types.SimpleNamespace(check=lambda: -7, args=(0, 0, 0, 0, 0, 1, 3, 0, 3, 64), kv_heads=2, head_dim=64, page_size=64, page_table=torch.zeros(1, 3, dtype=torch.int32))
+    i = torch.zeros(2, dtype=torch.int32)
+    for n in (1, 40):
+        q = torch.zeros(n, 14 * 64, dtype=torch.bfloat16)
+        for mask in (dict(window=(1 << 32) + 5), dict(window=3, keep_first=(1 << 31) - 1), dict(chunk=1 << 40), dict(window=1 << 31, keep_first=1 << 33)):
+            del seen[:]
+            bindings.attention_quantised(q, q, i, i, 1, n, 190, 14, kv, 0.125, **mask)
+            name, a = seen[0]
+            assert name == ("mlc_attention_q8" if n == 1 else "mlc_attention_q8_tcgen05")
+            assert a[11:14] == tuple(min(mask.get(k, 0), (1 << 31) - 256) for k in ("window", "keep_first", "chunk"))
+            assert all(x + 128 < 1 << 31 for x in a[11:14])
